@@ -28,6 +28,7 @@ extern "C" {
 
 #define RT_MAX_RANK 8
 #define RT_MAX_PEERS 8
+#define RT_MAX_SEGMENTS 3 /* most segments a dtype's buffer has */
 
 typedef enum rt_status {
     RT_OK = 0,
@@ -58,7 +59,14 @@ typedef enum rt_dtype {
     RT_U32 = 4,
     RT_Q8_0H = 5, /* GGUF Q8_0 split into codes | f16 scales */
     RT_Q8_0F = 6, /* GGUF Q8_0 split into codes | f32 scales */
-    RT_Q4_K = 7   /* raw GGUF Q4_K super-blocks, 144 bytes per 256 values */
+    RT_Q4_K = 7,  /* raw GGUF Q4_K super-blocks, 144 bytes per 256 values */
+    /* 4-bit codes with an f16 scale and a zero point per group of 32, 64 or 128 consecutive values of a row (an
+     * extension: the reference has no such format): value = (q - z) * s, exact in f32.  Operand of f16 and bf16
+     * activations.  Where the activations are many (a tensor-core GEMM) the values are rounded to f16 once, so
+     * |value| <= 65504 is the weight's part. */
+    RT_Q4_G32 = 8,
+    RT_Q4_G64 = 9,
+    RT_Q4_G128 = 10
 } rt_dtype;
 
 typedef enum rt_epilogue {
@@ -144,7 +152,9 @@ rt_status rt_dtype_activation(rt_dtype dt, rt_dtype *out); /* dtype/mod.rs:77-83
 /* DType::segments (dtype/mod.rs:85-95) / Q8_0<T>::segments (dtype/blocks.rs:61-74):
  * the byte ranges of one tensor's buffer.  Q8_0: codes then scales, each padded to 256 B.
  * Plain types: one segment of max(numel*size, 16) rounded up to 4 B.  Q4_K: one segment of
- * numel/256*144 bytes.  `segs` has room for *n_segs entries; *n_segs is set to the count. */
+ * numel/256*144 bytes.  Q4_G*: codes (two in a byte, the value of even index in the low half), f16
+ * scales, zero points (a byte each, its low five bits count: 0..31), each padded to 256 B, groups in
+ * the order of their values.  `segs` has room for *n_segs entries; *n_segs is set to the count. */
 rt_status rt_dtype_segments(rt_dtype dt, uint64_t numel, rt_segment *segs, int32_t *n_segs);
 /* Sum of the segment sizes: the bytes a tensor of this dtype occupies on the device. */
 rt_status rt_dtype_nbytes(rt_dtype dt, uint64_t numel, uint64_t *nbytes);
@@ -163,6 +173,12 @@ rt_status rt_transcode_gguf_q8_0(const void *blocks, uint64_t n_blocks, rt_dtype
  * counterpart for the arithmetic, which follows the published GGUF format). */
 rt_status rt_quantize_q4_k(const float *src, uint64_t numel, void *out);
 rt_status rt_dequantize_q4_k(const void *src, uint64_t numel, float *out);
+/* f32 -> a Q4_G* buffer (rt_dtype_nbytes(dt, numel) bytes; numel a multiple of the group): per group the
+ * affine fit between min(values, 0) and max(values, 0) in 15 steps, or with `symmetric` z = 8 and
+ * s = absmax / 7; s is rounded to f16 (at most 65504) before the codes are taken, codes round to nearest
+ * even and saturate, a NaN value takes the zero point's code. */
+rt_status rt_quantize_q4_group(const float *src, uint64_t numel, rt_dtype dt, int32_t symmetric, void *out);
+rt_status rt_dequantize_q4_group(const void *src, uint64_t numel, rt_dtype dt, float *out);
 
 /* ------------------------------------------------------------------ Matmul rules (host) */
 
@@ -365,6 +381,88 @@ typedef struct rt_mlp_desc {
 } rt_mlp_desc;
 rt_status rt_mlp_create(rt_device *dev, const rt_mlp_desc *mlp, int32_t use_graph, rt_executable **exe);
 
+/* ------------------------------------------------------------------ around the Linears of a decode step
+ * Operators that stand between Matmul nodes and behind the last one.  They need no plan and no
+ * scratch: a launch reads its description on the host and enqueues one kernel, so it can be captured
+ * into a graph and run on several streams at once.  `stream` NULL = the device's stream. */
+
+typedef enum rt_norm_kind {
+    RT_NORM_NONE = 0,
+    RT_NORM_RMS = 1,  /* v / sqrt(mean(v^2) + eps) * weight            (crates/ratchet-nn/src/norm.rs, RMSNorm) */
+    RT_NORM_LAYER = 2 /* (v - mean) / sqrt(var + eps) * weight + bias  (the same file, LayerNorm) */
+} rt_norm_kind;
+
+typedef struct rt_norm {
+    int32_t kind;       /* rt_norm_kind */
+    rt_dtype dt;        /* of weight and bias: RT_F32, or the activations' */
+    float eps;          /* >= 0 */
+    const void *weight; /* [d]; NULL = ones */
+    const void *bias;   /* [d], RT_NORM_LAYER only; NULL = none */
+} rt_norm;
+
+/* What stands between two blocks of a model, over rows of d values (1 .. RT_NORM_MAX_D):
+ *     h = residual_scale * residual + block_scale * gate * post(block)
+ *     x = pre(h)
+ * h is the new residual stream, x the next block's input.  Statistics and sums are f32 throughout, x is
+ * taken from h before h is rounded to dt.  residual NULL drops the first term, block NULL the second (a
+ * plain norm: residual = the input, residual_scale = 1, h = NULL); h NULL is not stored; pre.kind
+ * RT_NORM_NONE goes with x NULL.  A gate has gate_rows rows of d values (dense) and gate row i scales rows
+ * [i rows / gate_rows, (i + 1) rows / gate_rows); gate_rows divides rows (1: one gate for all).
+ * Rows of an operand start *_ld elements apart (>= d).  Each of h and x may be the memory of residual or of
+ * block, with the same ld; any other overlap of an output with another operand is refused (RT_ERR_INVARIANT). */
+#define RT_NORM_MAX_D 32768
+typedef struct rt_residual_norm {
+    rt_dtype dt; /* RT_F32, RT_F16 or RT_BF16 */
+    float residual_scale, block_scale;
+    int64_t rows, d;
+    const void *residual, *block;
+    int64_t residual_ld, block_ld;
+    const void *gate;
+    int64_t gate_rows; /* ignored without a gate */
+    rt_norm post, pre;
+    void *h, *x;
+    int64_t h_ld, x_ld;
+} rt_residual_norm;
+/* The checks of a description alone (host only). */
+rt_status rt_residual_norm_check(const rt_residual_norm *op);
+rt_status rt_residual_norm_launch(rt_device *dev, const rt_residual_norm *op, void *stream);
+
+/* What a step answers with, from its logits [rows][vocab] (rows ld elements apart):
+ *     log_prob[r] = v[token] - ln sum e^v          tokens[r] outside 0 .. vocab-1: NaN
+ *     entropy[r]  = - sum p ln p
+ *     top_ids, top_log_prob [rows][top]: the most likely tokens in falling order, equal logits by lower id
+ * A logit of -inf is a token that cannot be drawn; a row of nothing else gives -inf for every log
+ * probability and an entropy of 0.  A NaN or +inf makes its row's log probabilities and entropy NaN; top_ids
+ * then order NaN above +inf.  log_prob goes with tokens; it, entropy and the top outputs may each be left
+ * out (NULL, top = 0), not all of them.  f32 values, sums in f32 from at most a few thousand terms each. */
+#define RT_LOG_PROBS_MAX_TOP 32
+typedef struct rt_log_probs {
+    rt_dtype dt; /* RT_F32, RT_F16 or RT_BF16 */
+    int32_t top; /* 0 .. min(vocab, RT_LOG_PROBS_MAX_TOP) */
+    int64_t rows, vocab, ld;
+    const void *logits;
+    const int32_t *tokens;
+    float *log_prob, *entropy;
+    int32_t *top_ids;
+    float *top_log_prob;
+} rt_log_probs;
+rt_status rt_log_probs_check(const rt_log_probs *op);
+rt_status rt_log_probs_launch(rt_device *dev, const rt_log_probs *op, void *stream);
+
+/* rt_executable_create for lists that hold these operators beside Matmul nodes: one step per entry, in
+ * execution order, each with its operands bound.  Such a list is dispatched as a CUDA graph or, with
+ * use_graph = 0, launch by launch (a list of Matmul nodes only is rt_executable_create's). */
+typedef enum rt_step_kind { RT_STEP_MATMUL = 0, RT_STEP_RESIDUAL_NORM = 1, RT_STEP_LOG_PROBS = 2 } rt_step_kind;
+typedef struct rt_step {
+    int32_t kind; /* rt_step_kind: which of the members counts */
+    rt_dispatch matmul;
+    rt_residual_norm norm;
+    rt_log_probs log_probs;
+} rt_step;
+/* rt_abi_layout for the structs of this section. */
+int32_t rt_abi_layout_steps(uint64_t *out, int32_t n);
+rt_status rt_executable_create_steps(rt_device *dev, const rt_step *steps, int32_t n_steps, int32_t use_graph, rt_executable **exe);
+
 /* Linear-shaped Q8_0 GEMM for callers that must not allocate device memory: out[rows][n] =
  * x[rows][k] . W[n][k]^T (+ bias[n]) (+ GELU), W as RT_Q8_0H, x / bias / out f16 -- the node
  * W.gemm(x, b, false, true, true) of nn::Linear.  It has no counterpart in the reference.
@@ -403,7 +501,7 @@ rt_status rt_ipc_close(rt_device *dev, void *ptr);
  * ordinary tensor of shape [r1-r0][k] holding rt_dtype_nbytes(dt, (r1-r0)*k) bytes. */
 rt_status rt_shard_rows(rt_dtype dt, const void *src, uint64_t rows, uint64_t k, uint64_t r0, uint64_t r1, void *dst);
 
-/* Debug / parity helper: dequantise a device tensor into f32 (RT_Q8_0F, RT_Q4_K) or f16
+/* Debug / parity helper: dequantise a device tensor into f32 (RT_Q8_0F, RT_Q4_K, RT_Q4_G*) or f16
  * (RT_Q8_0H) exactly as the kernels decode it, so "bit-exact dequantised weights" can be
  * checked on the device.  Arithmetic: quant.rs:114-120; gemm.rs:400-406 for the f16 form. */
 rt_status rt_dequantize_device(rt_device *dev, rt_dtype dt, uint64_t numel, const void *src, void *dst, void *stream);

@@ -12,9 +12,10 @@ from ._lib import RT_EPILOGUE_SILU_MUL as EPILOGUE_SILU_MUL
 from .tensor import (Device, DeviceRequest, DType, Executable, GpuBuffer, Linear, Matmul, MLP, PinnedArray, Quantization, Quantizer,
                      Tensor, bf16_bits_to_f32, f32_to_bf16_bits, transcode_gguf_q8_0)
 
+from .ops import LayerNorm, LogProbs, ResidualNorm, RMSNorm
 from .sharded import Comm, ShardedLinear, shard_bounds, shard_rows
 from .gguf import GGUF, TensorInfo
 
 __all__ = ["GGUF", "TensorInfo", "Comm", "ShardedLinear", "shard_bounds", "shard_rows", "Device", "DeviceRequest", "DType", "Executable", "GpuBuffer", "Linear", "Matmul", "PinnedArray", "Quantization",
            "Quantizer", "Tensor", "RatchetError", "ShapeError", "InvariantError", "EPILOGUE_NONE",
-           "EPILOGUE_GELU_TANH", "EPILOGUE_SILU_MUL", "MLP", "bf16_bits_to_f32", "f32_to_bf16_bits", "transcode_gguf_q8_0"]
+           "EPILOGUE_GELU_TANH", "EPILOGUE_SILU_MUL", "MLP", "LayerNorm", "LogProbs", "ResidualNorm", "RMSNorm", "bf16_bits_to_f32", "f32_to_bf16_bits", "transcode_gguf_q8_0"]

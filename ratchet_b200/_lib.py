@@ -20,10 +20,13 @@ RT_OK, RT_ERR_SHAPE, RT_ERR_DTYPE, RT_ERR_INVARIANT, RT_ERR_ARG, RT_ERR_CUDA, RT
     RT_ERR_NOMEM, RT_ERR_COMM, RT_ERR_COMM_TIMEOUT = range(10)
 
 # rt_dtype
-RT_F32, RT_F16, RT_BF16, RT_I32, RT_U32, RT_Q8_0H, RT_Q8_0F, RT_Q4_K = range(8)
+RT_F32, RT_F16, RT_BF16, RT_I32, RT_U32, RT_Q8_0H, RT_Q8_0F, RT_Q4_K, RT_Q4_G32, RT_Q4_G64, RT_Q4_G128 = range(11)
 
 RT_EPILOGUE_NONE, RT_EPILOGUE_GELU_TANH, RT_EPILOGUE_SILU_MUL = 0, 1, 2
 RT_LAUNCH_LHS_CONSTANT = 1
+
+RT_NORM_NONE, RT_NORM_RMS, RT_NORM_LAYER = 0, 1, 2
+RT_STEP_MATMUL, RT_STEP_RESIDUAL_NORM, RT_STEP_LOG_PROBS = 0, 1, 2
 
 
 class rt_shape(Structure):
@@ -85,6 +88,26 @@ class rt_mlp_desc(Structure):
                 ("w2", c_void_p), ("b2", c_void_p), ("x", c_void_p), ("out", c_void_p)]
 
 
+class rt_norm(Structure):
+    _fields_ = [("kind", c_int32), ("dt", c_int32), ("eps", c_float), ("weight", c_void_p), ("bias", c_void_p)]
+
+
+class rt_residual_norm(Structure):
+    _fields_ = [("dt", c_int32), ("residual_scale", c_float), ("block_scale", c_float), ("rows", c_int64), ("d", c_int64),
+                ("residual", c_void_p), ("block", c_void_p), ("residual_ld", c_int64), ("block_ld", c_int64),
+                ("gate", c_void_p), ("gate_rows", c_int64), ("post", rt_norm), ("pre", rt_norm),
+                ("h", c_void_p), ("x", c_void_p), ("h_ld", c_int64), ("x_ld", c_int64)]
+
+
+class rt_log_probs(Structure):
+    _fields_ = [("dt", c_int32), ("top", c_int32), ("rows", c_int64), ("vocab", c_int64), ("ld", c_int64), ("logits", c_void_p),
+                ("tokens", c_void_p), ("log_prob", c_void_p), ("entropy", c_void_p), ("top_ids", c_void_p), ("top_log_prob", c_void_p)]
+
+
+class rt_step(Structure):
+    _fields_ = [("kind", c_int32), ("matmul", rt_dispatch), ("norm", rt_residual_norm), ("log_probs", rt_log_probs)]
+
+
 class rt_gguf_value(Structure):
     _fields_ = [("type", c_int32), ("elem_type", c_int32), ("len", c_uint64), ("u64", c_uint64),
                 ("i64", c_int64), ("f64", ctypes.c_double), ("str", c_void_p), ("node", c_void_p)]
@@ -141,6 +164,8 @@ def load() -> ctypes.CDLL:
         "rt_transcode_gguf_q8_0": (c_int32, [V, c_uint64, c_int32, V]),
         "rt_quantize_q4_k": (c_int32, [V, c_uint64, V]),
         "rt_dequantize_q4_k": (c_int32, [V, c_uint64, V]),
+        "rt_quantize_q4_group": (c_int32, [V, c_uint64, c_int32, c_int32, V]),
+        "rt_dequantize_q4_group": (c_int32, [V, c_uint64, c_int32, V]),
         "rt_matmul_spec": (c_int32, [POINTER(rt_matmul_desc), POINTER(rt_gemm_spec)]),
         "rt_matmul_out_shape": (c_int32, [POINTER(rt_matmul_desc), POINTER(rt_shape)]),
         "rt_device_create": (c_int32, [c_int32, POINTER(V)]),
@@ -174,6 +199,12 @@ def load() -> ctypes.CDLL:
         "rt_executable_arena": (c_int32, [V, POINTER(c_uint64), POINTER(c_int32), POINTER(c_uint64)]),
         "rt_executable_tensor": (V, [V, c_int32]),
         "rt_mlp_create": (c_int32, [V, POINTER(rt_mlp_desc), c_int32, POINTER(V)]),
+        "rt_residual_norm_check": (c_int32, [POINTER(rt_residual_norm)]),
+        "rt_residual_norm_launch": (c_int32, [V, POINTER(rt_residual_norm), V]),
+        "rt_log_probs_check": (c_int32, [POINTER(rt_log_probs)]),
+        "rt_log_probs_launch": (c_int32, [V, POINTER(rt_log_probs), V]),
+        "rt_abi_layout_steps": (c_int32, [POINTER(c_uint64), c_int32]),
+        "rt_executable_create_steps": (c_int32, [V, POINTER(rt_step), c_int32, c_int32, POINTER(V)]),
         "rt_arena_plan": (c_int32, [POINTER(rt_usage_record), c_int32, c_uint64, POINTER(c_int32), POINTER(c_uint64),
                                     POINTER(c_int32), POINTER(c_uint64)]),
         "rt_executable_dispatch": (c_int32, [V, V]),

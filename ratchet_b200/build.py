@@ -20,6 +20,7 @@ SOURCES = [
     "spec.cpp",
     "arena.cpp",
     "quant_host.cpp",
+    "decode_ops.cpp",
     "gguf_reader.cpp",
     "comm.cpp",
     "api.cu",
@@ -29,6 +30,7 @@ SOURCES = [
     "gemv_q4k_mma.cu", "gemv_q4k_umma.cu",
     "gemv_q8f_f32.cu", "gemv_q4k_f16.cu",
     "dequant.cu",
+    "residual_norm.cu", "log_probs.cu",
     "gemm_umma.cu", "gemm_umma_tf32.cu",
     "static_scratch.cu",
 ]

@@ -15,17 +15,19 @@
 #include <vector>
 
 #include "arena.hpp"
+#include "decode_ops.hpp"
 #include "kernels.hpp"
 #include "ratchet_b200.h"
 #include "spec.hpp"
 
 namespace rt {
-Status dtype_segments(rt_dtype dt, uint64_t numel, rt_segment *segs, int *n);
 Status quantize_q8_0(const float *x, uint64_t numel, rt_dtype dt, uint8_t *out);
 Status dequantize_q8_0(const uint8_t *src, uint64_t numel, rt_dtype dt, float *out);
 Status transcode_gguf_q8_0(const uint8_t *blocks, uint64_t n_blocks, rt_dtype dt, uint8_t *out);
 Status quantize_q4_k(const float *x, uint64_t numel, uint8_t *out);
 Status dequantize_q4_k(const uint8_t *src, uint64_t numel, float *out);
+Status quantize_q4_group(const float *x, uint64_t numel, rt_dtype dt, bool symmetric, uint8_t *out);
+Status dequantize_q4_group(const uint8_t *src, uint64_t numel, rt_dtype dt, float *out);
 } // namespace rt
 
 using namespace rt;
@@ -84,7 +86,7 @@ struct rt_plan {
     int nv2 = 0;           // streaming Q8_0 kernel: vectors beyond the first launch's 8, taken 8 at a time (9..24 in all)
     bool chain_ok = false; // a Q8_0H x f16 GEMV the persistent chain kernel can take as a node
     MatmulParams params{}; // everything but the pointers
-    uint64_t lhs_scale_offset = 0;
+    uint64_t lhs_scale_offset = 0, lhs_zero_offset = 0;
     // tensor-core GEMM: operand roles, tile width, and the scratch that holds dequantised weights
     bool lhs_is_q = false; // the lhs is the kernel's Q operand (trans_out), else its P operand
     int R = 0, S = 0, u_stacks = 1, p_stack = 1, q_stack = 1, bn = 128, ksplit = 1;
@@ -192,6 +194,7 @@ struct ScratchSet {
 struct rt_executable {
     rt_device *dev = nullptr;
     std::vector<rt_dispatch> nodes;
+    std::vector<rt_step> steps; // rt_executable_create_steps: the execution order, Matmul steps standing for `nodes` in turn; else empty
     // One allocation for every intermediate tensor and every node's plan scratch, placed by the activation planner
     // (arena.cpp, the reference's BufferAllocator::greedy_by_size).
     std::vector<ScratchSet> scratch; // per node: where its plan's scratch areas live in the arena
@@ -292,7 +295,7 @@ rt_status rt_dtype_activation(rt_dtype dt, rt_dtype *out) {
 
 rt_status rt_dtype_segments(rt_dtype dt, uint64_t numel, rt_segment *segs, int32_t *n_segs) {
     if (!segs || !n_segs || !dtype_valid(dt)) return fail(RT_ERR_ARG, "rt_dtype_segments: bad argument");
-    rt_segment tmp[2];
+    rt_segment tmp[RT_MAX_SEGMENTS];
     int n = 0;
     Status st = dtype_segments(dt, numel, tmp, &n);
     if (!st.ok()) return fail(st);
@@ -304,7 +307,7 @@ rt_status rt_dtype_segments(rt_dtype dt, uint64_t numel, rt_segment *segs, int32
 
 rt_status rt_dtype_nbytes(rt_dtype dt, uint64_t numel, uint64_t *nbytes) {
     if (!nbytes || !dtype_valid(dt)) return fail(RT_ERR_ARG, "rt_dtype_nbytes: bad argument");
-    rt_segment tmp[2];
+    rt_segment tmp[RT_MAX_SEGMENTS];
     int n = 0;
     Status st = dtype_segments(dt, numel, tmp, &n);
     if (!st.ok()) return fail(st);
@@ -342,6 +345,18 @@ rt_status rt_quantize_q4_k(const float *src, uint64_t numel, void *out) {
 rt_status rt_dequantize_q4_k(const void *src, uint64_t numel, float *out) {
     if (!src || !out) return fail(RT_ERR_ARG, "rt_dequantize_q4_k: bad argument");
     Status st = dequantize_q4_k((const uint8_t *)src, numel, out);
+    return st.ok() ? RT_OK : fail(st);
+}
+
+rt_status rt_quantize_q4_group(const float *src, uint64_t numel, rt_dtype dt, int32_t symmetric, void *out) {
+    if (!src || !out || q4_group(dt) == 0) return fail(RT_ERR_ARG, "rt_quantize_q4_group: bad argument");
+    Status st = quantize_q4_group(src, numel, dt, symmetric != 0, (uint8_t *)out);
+    return st.ok() ? RT_OK : fail(st);
+}
+
+rt_status rt_dequantize_q4_group(const void *src, uint64_t numel, rt_dtype dt, float *out) {
+    if (!src || !out || q4_group(dt) == 0) return fail(RT_ERR_ARG, "rt_dequantize_q4_group: bad argument");
+    Status st = dequantize_q4_group((const uint8_t *)src, numel, dt, out);
     return st.ok() ? RT_OK : fail(st);
 }
 
@@ -627,13 +642,15 @@ static bool umma_eligible(const rt_matmul_desc &d, const Spec &s) {
     } else {
         if (d.rhs_dt != RT_F16 && d.rhs_dt != RT_BF16) return false;
         const bool dense = d.lhs_dt == d.rhs_dt;
-        if (!dense && d.lhs_dt != RT_Q8_0H && d.lhs_dt != RT_Q4_K) return false;
+        if (!dense && d.lhs_dt != RT_Q8_0H && d.lhs_dt != RT_Q4_K && q4_group(d.lhs_dt) == 0) return false;
         // a dense 16-bit product with rhs [K][N] whose K is not a multiple of 8 (Whisper's softmax.v, K = 1500):
         // both operands are repacked anyway or cheaply, with K zero-padded to the next multiple of 8
         const long long k_eff = (!s.trans_rhs && dense) ? (s.K + 7) / 8 * 8 : s.K;
         if (!umma_gemm_supported(k_eff)) return false;
     }
-    if (s.M < 1 || s.N < 9 || s.stacks < 1) return false; // up to 8 columns: the streaming GEMV kernels
+    // (a batch of single rows against one 4-bit group weight counts as that many columns: the GEMM flattens it anyway)
+    const int64_t columns = q4_group(d.lhs_dt) != 0 && s.trans_out && s.lhs_stack == 1 ? s.stacks * s.N : s.N;
+    if (s.M < 1 || columns < 9 || s.stacks < 1) return false; // up to 8 columns: the streaming GEMV kernels
     if ((double)s.M * (double)s.N * (double)s.K * (double)s.stacks < (double)(1 << 21)) return false;
     return true;
 }
@@ -688,8 +705,20 @@ static rt_status build_plan(rt_device *dev, const rt_matmul_desc *desc, rt_plan 
     p.lhs_batch_elems = s.M * s.K;
     p.lhs_batch_scale_bytes = 0;
     pl->lhs_scale_offset = 0;
+    if (const int group = q4_group(desc->lhs_dt); group != 0) {
+        rt_segment seg[RT_MAX_SEGMENTS];
+        int n = 0;
+        st = dtype_segments(desc->lhs_dt, (uint64_t)(s.lhs_stack * s.M * s.K), seg, &n);
+        if (!st.ok()) {
+            delete pl;
+            return fail(st);
+        }
+        pl->lhs_scale_offset = seg[1].offset;
+        pl->lhs_zero_offset = seg[2].offset;
+        p.lhs_group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
+    }
     if (desc->lhs_dt == RT_Q8_0H || desc->lhs_dt == RT_Q8_0F) {
-        rt_segment seg[2];
+        rt_segment seg[RT_MAX_SEGMENTS];
         int n = 0;
         st = dtype_segments(desc->lhs_dt, (uint64_t)(s.lhs_stack * s.M * s.K), seg, &n);
         if (!st.ok()) {
@@ -985,6 +1014,21 @@ int32_t rt_abi_layout(uint64_t *out, int32_t n) {
     return count;
 }
 
+// The same for the operators around the Linears:
+// {sizeof(rt_norm), offsetof weight, sizeof(rt_residual_norm), offsetof rows, gate, post, h, x_ld, sizeof(rt_log_probs), offsetof
+//  rows, logits, top_log_prob, sizeof(rt_step), offsetof matmul, norm, log_probs}
+int32_t rt_abi_layout_steps(uint64_t *out, int32_t n) {
+    const uint64_t v[] = {
+        sizeof(rt_norm), offsetof(rt_norm, weight),
+        sizeof(rt_residual_norm), offsetof(rt_residual_norm, rows), offsetof(rt_residual_norm, gate), offsetof(rt_residual_norm, post),
+        offsetof(rt_residual_norm, h), offsetof(rt_residual_norm, x_ld),
+        sizeof(rt_log_probs), offsetof(rt_log_probs, rows), offsetof(rt_log_probs, logits), offsetof(rt_log_probs, top_log_prob),
+        sizeof(rt_step), offsetof(rt_step, matmul), offsetof(rt_step, norm), offsetof(rt_step, log_probs)};
+    const int32_t count = (int32_t)(sizeof(v) / sizeof(v[0]));
+    for (int32_t i = 0; i < count && i < n; i++) out[i] = v[i];
+    return count;
+}
+
 rt_status rt_plan_spec(const rt_plan *plan, rt_gemm_spec *spec) {
     if (!plan || !spec) return fail(RT_ERR_ARG, "rt_plan_spec: null argument");
     fill_public_spec(plan->spec, spec);
@@ -998,6 +1042,7 @@ static MatmulParams bound_params(const rt_plan *plan, const void *lhs, const voi
     MatmulParams p = plan->params;
     p.lhs = lhs;
     p.lhs_scales = plan->lhs_scale_offset ? (const void *)((const char *)lhs + plan->lhs_scale_offset) : nullptr;
+    p.lhs_zeros = plan->lhs_zero_offset ? (const uint8_t *)lhs + plan->lhs_zero_offset : nullptr;
     p.rhs = rhs;
     p.bias = plan->spec.has_bias ? bias : nullptr;
     p.out = out;
@@ -1038,7 +1083,7 @@ rt_status rt_graph_resolve(rt_device *dev, const uint64_t *nodes, int32_t n, uin
                 operand[k] = reinterpret_cast<const void *>(v);
             }
         }
-        rt_segment seg[2];
+        rt_segment seg[RT_MAX_SEGMENTS];
         int nseg = 0;
         uint64_t bytes = 0;
         Status st = dtype_segments(plan->spec.out_dt, (uint64_t)numel(plan->spec.out_shape), seg, &nseg);
@@ -1246,14 +1291,29 @@ static rt_status launch_node(rt_plan *plan, const void *lhs, const void *rhs, co
 extern "C" {
 
 
+static rt_status dispatch_node(rt_executable *exe, size_t i, cudaStream_t st) {
+    const rt_dispatch &n = exe->nodes[i];
+    return launch_node(n.plan, n.lhs, n.rhs, n.bias, n.out, (void *)st, &n.opts, &exe->scratch[i]);
+}
+
 static rt_status dispatch_nodes(rt_executable *exe, cudaStream_t st) {
-    for (size_t i = 0; i < exe->nodes.size(); i++) {
-        const rt_dispatch &n = exe->nodes[i];
-        rt_status s = launch_node(n.plan, n.lhs, n.rhs, n.bias, n.out, (void *)st, &n.opts, &exe->scratch[i]);
+    if (exe->steps.empty()) {
+        for (size_t i = 0; i < exe->nodes.size(); i++)
+            if (rt_status s = dispatch_node(exe, i, st); s != RT_OK) return s;
+        return RT_OK;
+    }
+    size_t node = 0;
+    for (const rt_step &step : exe->steps) {
+        const rt_status s = step.kind == RT_STEP_MATMUL          ? dispatch_node(exe, node++, st)
+                            : step.kind == RT_STEP_RESIDUAL_NORM ? rt_residual_norm_launch(exe->dev, &step.norm, (void *)st)
+                                                                 : rt_log_probs_launch(exe->dev, &step.log_probs, (void *)st);
         if (s != RT_OK) return s;
     }
     return RT_OK;
 }
+
+static rt_status create_executable(rt_device *dev, const rt_dispatch *nodes, const rt_node_tensors *ids, int32_t n_nodes, const uint64_t *tensor_bytes,
+                                   int32_t n_tensors, std::vector<rt_step> steps, int32_t use_graph, rt_executable **exe);
 
 rt_status rt_executable_create(rt_device *dev, const rt_dispatch *nodes, int32_t n_nodes, int32_t use_graph, rt_executable **exe) {
     return rt_executable_create_planned(dev, nodes, nullptr, n_nodes, nullptr, 0, use_graph, exe);
@@ -1263,6 +1323,28 @@ rt_status rt_executable_create_planned(rt_device *dev, const rt_dispatch *nodes,
                                        const uint64_t *tensor_bytes, int32_t n_tensors, int32_t use_graph, rt_executable **exe) {
     if (!dev || !exe || (n_nodes > 0 && !nodes) || n_nodes < 0 || n_tensors < 0 || (n_tensors > 0 && (!tensor_bytes || !ids)))
         return fail(RT_ERR_ARG, "rt_executable_create: bad argument");
+    return create_executable(dev, nodes, ids, n_nodes, tensor_bytes, n_tensors, {}, use_graph, exe);
+}
+
+rt_status rt_executable_create_steps(rt_device *dev, const rt_step *steps, int32_t n_steps, int32_t use_graph, rt_executable **exe) {
+    if (!dev || !exe || n_steps < 0 || (n_steps > 0 && !steps)) return fail(RT_ERR_ARG, "rt_executable_create_steps: bad argument");
+    std::vector<rt_dispatch> nodes;
+    for (int32_t i = 0; i < n_steps; i++) {
+        Status st = Status::Ok();
+        switch (steps[i].kind) {
+        case RT_STEP_MATMUL: nodes.push_back(steps[i].matmul); break;
+        case RT_STEP_RESIDUAL_NORM: st = check_residual_norm(steps[i].norm); break;
+        case RT_STEP_LOG_PROBS: st = check_log_probs(steps[i].log_probs); break;
+        default: return fail(RT_ERR_ARG, "rt_executable_create_steps: invalid step kind");
+        }
+        if (!st.ok()) return fail(st);
+    }
+    if ((size_t)n_steps == nodes.size()) return create_executable(dev, nodes.data(), nullptr, n_steps, nullptr, 0, {}, use_graph, exe);
+    return create_executable(dev, nodes.data(), nullptr, (int32_t)nodes.size(), nullptr, 0, std::vector<rt_step>(steps, steps + n_steps), use_graph, exe);
+}
+
+static rt_status create_executable(rt_device *dev, const rt_dispatch *nodes, const rt_node_tensors *ids, int32_t n_nodes, const uint64_t *tensor_bytes,
+                                   int32_t n_tensors, std::vector<rt_step> steps, int32_t use_graph, rt_executable **exe) {
     std::unique_ptr<rt_executable> x(new (std::nothrow) rt_executable());
     if (!x) return fail(RT_ERR_NOMEM, "out of host memory");
     x->dev = dev;
@@ -1272,6 +1354,9 @@ rt_status rt_executable_create_planned(rt_device *dev, const rt_dispatch *nodes,
         x->nodes.push_back(nodes[i]);
         x->launches += nodes[i].plan->launches;
     }
+    for (const rt_step &step : steps)
+        if (step.kind != RT_STEP_MATMUL && (step.kind == RT_STEP_RESIDUAL_NORM ? step.norm.rows : step.log_probs.rows) > 0) x->launches += 1;
+    x->steps = std::move(steps);
     x->scratch.resize((size_t)n_nodes);
     x->tensors.assign((size_t)n_tensors, nullptr);
 
@@ -1295,7 +1380,7 @@ rt_status rt_executable_create_planned(rt_device *dev, const rt_dispatch *nodes,
             if (x->nodes[(size_t)i].opts.n_out > 0)
                 return fail(RT_ERR_ARG, "rt_executable_create: a scattered output cannot be an intermediate");
             const Spec &sp = x->nodes[(size_t)i].plan->spec;
-            rt_segment seg[2];
+            rt_segment seg[RT_MAX_SEGMENTS];
             int nseg = 0;
             uint64_t need = 0;
             Status st = dtype_segments(sp.out_dt, (uint64_t)numel(sp.out_shape), seg, &nseg);
@@ -1378,7 +1463,7 @@ rt_status rt_executable_create_planned(rt_device *dev, const rt_dispatch *nodes,
             return fail(RT_ERR_INVARIANT, "Matmul is never in place: out aliases an operand");
 
     // A list of tensor-memory Q8_0 GEMVs over constant weights runs as one persistent kernel.
-    if (use_graph && n_nodes >= 2 && chain_enabled()) {
+    if (use_graph && n_nodes >= 2 && chain_enabled() && x->steps.empty()) {
         bool all = true;
         std::vector<MatmulParams> ps;
         for (const rt_dispatch &n : x->nodes) {
@@ -1459,7 +1544,7 @@ rt_status rt_mlp_create(rt_device *dev, const rt_mlp_desc *mlp, int32_t use_grap
         return fail(RT_ERR_SHAPE, "rt_mlp_create: fc1 produces " + dims_str(hid) + " " + dtype_name(p1->spec.out_dt) + ", fc2 takes " +
                                       dims_str(rhs2) + " " + dtype_name(mlp->fc2.rhs_dt));
     }
-    rt_segment seg[2];
+    rt_segment seg[RT_MAX_SEGMENTS];
     int nseg = 0;
     uint64_t hidden_bytes = 0;
     Status st = dtype_segments(p1->spec.out_dt, (uint64_t)numel(hid), seg, &nseg);
@@ -1509,18 +1594,46 @@ rt_status rt_executable_destroy(rt_executable *exe) {
     return RT_OK;
 }
 
+rt_status rt_residual_norm_check(const rt_residual_norm *op) {
+    if (!op) return fail(RT_ERR_ARG, "rt_residual_norm: null argument");
+    Status st = check_residual_norm(*op);
+    return st.ok() ? RT_OK : fail(st);
+}
+
+rt_status rt_residual_norm_launch(rt_device *dev, const rt_residual_norm *op, void *stream) {
+    if (!dev) return fail(RT_ERR_ARG, "rt_residual_norm: null device");
+    if (rt_status s = rt_residual_norm_check(op); s != RT_OK || op->rows == 0) return s;
+    CUDA_TRY(cudaSetDevice(dev->ordinal));
+    CUDA_TRY(launch_residual_norm(*op, dev->sm_count, stream ? (cudaStream_t)stream : dev->stream));
+    return RT_OK;
+}
+
+rt_status rt_log_probs_check(const rt_log_probs *op) {
+    if (!op) return fail(RT_ERR_ARG, "rt_log_probs: null argument");
+    Status st = check_log_probs(*op);
+    return st.ok() ? RT_OK : fail(st);
+}
+
+rt_status rt_log_probs_launch(rt_device *dev, const rt_log_probs *op, void *stream) {
+    if (!dev) return fail(RT_ERR_ARG, "rt_log_probs: null device");
+    if (rt_status s = rt_log_probs_check(op); s != RT_OK || op->rows == 0) return s;
+    CUDA_TRY(cudaSetDevice(dev->ordinal));
+    CUDA_TRY(launch_log_probs(*op, dev->sm_count, stream ? (cudaStream_t)stream : dev->stream));
+    return RT_OK;
+}
+
 int32_t rt_executable_launches(const rt_executable *exe) { return exe ? exe->launches : 0; }
 const char *rt_executable_kernel(const rt_executable *exe) { return exe ? exe->how.c_str() : ""; }
 
 rt_status rt_dequantize_device(rt_device *dev, rt_dtype dt, uint64_t numel, const void *src, void *dst, void *stream) {
     if (!dev || !src || !dst) return fail(RT_ERR_ARG, "rt_dequantize_device: null argument");
     if (!dtype_valid(dt) || !is_quantized(dt)) return fail(RT_ERR_DTYPE, "rt_dequantize_device: not a block format");
-    rt_segment seg[2];
+    rt_segment seg[RT_MAX_SEGMENTS];
     int n = 0;
     Status st = dtype_segments(dt, numel, seg, &n);
     if (!st.ok()) return fail(st);
     CUDA_TRY(cudaSetDevice(dev->ordinal));
-    const void *scales = n == 2 ? (const void *)((const char *)src + seg[1].offset) : nullptr;
+    const void *scales = n >= 2 ? (const void *)((const char *)src + seg[1].offset) : nullptr;
     cudaStream_t s = stream ? (cudaStream_t)stream : dev->stream;
     CUDA_TRY(launch_dequant(dt, (long long)numel, src, scales, dst, dt == RT_Q8_0H ? RT_F16 : RT_F32, dev->sm_count, s));
     return RT_OK;

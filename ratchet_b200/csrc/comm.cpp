@@ -198,7 +198,7 @@ rt_status rt_ipc_close(rt_device *dev, void *ptr) {
 // padding, the rows' scales, padding), so that a shard is an ordinary tensor of shape [r1-r0][k].
 rt_status rt_shard_rows(rt_dtype dt, const void *src, uint64_t rows, uint64_t k, uint64_t r0, uint64_t r1, void *dst) {
     if (!src || !dst || r0 > r1 || r1 > rows || !dtype_valid(dt)) return fail(RT_ERR_ARG, "rt_shard_rows: bad argument");
-    rt_segment full[2], part[2];
+    rt_segment full[RT_MAX_SEGMENTS], part[RT_MAX_SEGMENTS];
     int nf = 0, np = 0;
     Status st = dtype_segments(dt, rows * k, full, &nf);
     if (st.ok()) st = dtype_segments(dt, (r1 - r0) * k, part, &np);
@@ -220,6 +220,16 @@ rt_status rt_shard_rows(rt_dtype dt, const void *src, uint64_t rows, uint64_t k,
         if (k % 256) return fail(RT_ERR_SHAPE, "Q4_K rows hold a multiple of 256 values");
         std::memcpy(d, s + r0 * (k / 256) * 144, n / 256 * 144);
         break;
+    case RT_Q4_G32:
+    case RT_Q4_G64:
+    case RT_Q4_G128: {
+        const uint64_t group = (uint64_t)q4_group(dt);
+        if (k % group) return fail(RT_ERR_SHAPE, std::string(dtype_name(dt)) + " rows hold a multiple of " + std::to_string(group) + " values");
+        std::memcpy(d, s + r0 * k / 2, n / 2);
+        std::memcpy(d + part[1].offset, s + full[1].offset + r0 * (k / group) * 2, n / group * 2);
+        std::memcpy(d + part[2].offset, s + full[2].offset + r0 * (k / group), n / group);
+        break;
+    }
     default:
         std::memcpy(d, s + r0 * k * dtype_size(dt), n * dtype_size(dt));
     }

@@ -20,7 +20,9 @@ enum BiasMode : int { BIAS_NONE = 0, BIAS_PER_N = 1, BIAS_PER_M = 2 };
 // trans_out.  Batch b reads lhs[b % lhs_stack] and rhs[b % rhs_stack] (gemm.rs:359-361).
 struct MatmulParams {
     const void *lhs;        // codes / values of the lhs
-    const void *lhs_scales; // Q8_0: scales segment (lhs + align256(numel)); else null
+    const void *lhs_scales; // Q8_0, Q4_G: scales segment; else null
+    const uint8_t *lhs_zeros; // Q4_G: zero points; else null
+    int lhs_group_shift;    // Q4_G: log2 of the values per group
     const void *rhs;
     const void *bias;
     void *out;

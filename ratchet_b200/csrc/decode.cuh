@@ -4,12 +4,13 @@
 //   Q8_0H  f16(q) * d rounded to f16            crates/ratchet-core/src/ops/gemm.rs:400-406
 //   Q4_K   (d*sc)*q - (dmin*m), separate f32 roundings (GGUF Q4_K; block struct
 //          crates/ratchet-loader/src/k_quants.rs:95-103)
+//   Q4_G   (q - z) * s: a five-bit whole number times an f16, exact in f32
 #pragma once
 #include "common.cuh"
 
 namespace rt {
 
-enum LhsKind : int { LK_F32 = 0, LK_F16 = 1, LK_BF16 = 2, LK_Q8H = 3, LK_Q8F = 4, LK_Q4K = 5 };
+enum LhsKind : int { LK_F32 = 0, LK_F16 = 1, LK_BF16 = 2, LK_Q8H = 3, LK_Q8F = 4, LK_Q4K = 5, LK_Q4G = 6 };
 
 __device__ __forceinline__ void q4k_scale_min(int j, const uint8_t *s, int &sc, int &m) {
     if (j < 4) {
@@ -38,7 +39,7 @@ __device__ __forceinline__ float q4k_element(const uint8_t *base, long long idx)
 
 // Value of lhs element at flat index `idx` (row-major within one batch slice).
 template <int KIND>
-__device__ __forceinline__ float lhs_element(const void *lhs, const void *scales, long long idx) {
+__device__ __forceinline__ float lhs_element(const void *lhs, const void *scales, long long idx, const uint8_t *zeros = nullptr, int group_shift = 0) {
     if (KIND == LK_F32) return ((const float *)lhs)[idx];
     if (KIND == LK_F16) return __half2float(((const __half *)lhs)[idx]);
     if (KIND == LK_BF16) return __bfloat162float(((const __nv_bfloat16 *)lhs)[idx]);
@@ -50,6 +51,11 @@ __device__ __forceinline__ float lhs_element(const void *lhs, const void *scales
     if (KIND == LK_Q8F) {
         const float q = (float)((const int8_t *)lhs)[idx];
         return __fmul_rn(q, ((const float *)scales)[idx >> 5]);
+    }
+    if (KIND == LK_Q4G) {
+        const long long group = idx >> group_shift;
+        const int q = ((const uint8_t *)lhs)[idx >> 1] >> (4 * (int)(idx & 1)) & 15;
+        return __fmul_rn((float)(q - (zeros[group] & 31)), __half2float(((const __half *)scales)[group]));
     }
     return q4k_element((const uint8_t *)lhs, idx);
 }

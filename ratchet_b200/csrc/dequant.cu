@@ -5,6 +5,7 @@
 
 #include "decode.cuh"
 #include "kernels.hpp"
+#include "spec.hpp"
 
 namespace rt {
 
@@ -36,6 +37,42 @@ __global__ void __launch_bounds__(256) dequant_q8h_f16_vec_kernel(const uint4 *c
         for (int j = 0; j < 8; j++) h[j] = __hmul2(h[j], d); // f16(q) * d rounded to f16
         dst[2 * i] = make_uint4(h2_as_u32(h[0]), h2_as_u32(h[1]), h2_as_u32(h[2]), h2_as_u32(h[3]));
         dst[2 * i + 1] = make_uint4(h2_as_u32(h[4]), h2_as_u32(h[5]), h2_as_u32(h[6]), h2_as_u32(h[7]));
+    }
+}
+
+// Q4_G -> f16 / f32, 32 values (16 code bytes, never more than one group) per thread: (q - z) * s is exact in f32 and rounded
+// once.  Accesses are 16 bytes where the pointers allow it.
+template <typename OutT>
+__global__ void __launch_bounds__(256) dequant_q4g_kernel(const uint8_t *codes, const __half *scales, const uint8_t *zeros, OutT *dst, long long n32,
+                                                          int group_shift) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool aligned = (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(dst)) % 16 == 0;
+    const long long stride = (long long)gridDim.x * blockDim.x;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n32; i += stride) {
+        const long long group = i >> (group_shift - 5);
+        const float s = __half2float(scales[group]);
+        const int z = zeros[group] & 31;
+        uint32_t w[4];
+        if (aligned) {
+            *reinterpret_cast<uint4 *>(w) = __ldg(reinterpret_cast<const uint4 *>(codes) + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint8_t *b = codes + i * 16 + j * 4;
+                w[j] = b[0] | b[1] << 8 | b[2] << 16 | (uint32_t)b[3] << 24;
+            }
+        }
+        alignas(16) OutT v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = from_f32<OutT>(__fmul_rn((float)((int)(w[j >> 3] >> (4 * (j & 7)) & 15u) - z), s));
+        if (aligned) {
+#pragma unroll
+            for (int j = 0; j < (int)(2 * sizeof(OutT)); j++) reinterpret_cast<uint4 *>(dst + i * 32)[j] = reinterpret_cast<const uint4 *>(v)[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++) dst[i * 32 + j] = v[j];
+        }
     }
 }
 
@@ -315,6 +352,18 @@ cudaError_t launch_dequant(rt_dtype dt, long long numel, const void *src, const 
         } else {
             dequant_kernel<LK_Q4K, __half><<<blocks, threads, 0, stream>>>(src, scales, (__half *)dst, numel);
         }
+    } else if (q4_group(dt) != 0 && (out_dt == RT_F16 || out_dt == RT_F32)) {
+        rt_segment seg[RT_MAX_SEGMENTS];
+        int n = 0;
+        if (!dtype_segments(dt, (uint64_t)numel, seg, &n).ok()) return cudaErrorInvalidValue;
+        const uint8_t *codes = (const uint8_t *)src, *zeros = codes + seg[2].offset;
+        const __half *s16 = (const __half *)(codes + seg[1].offset);
+        const int shift = q4_group(dt) == 32 ? 5 : q4_group(dt) == 64 ? 6 : 7;
+        const long long n32 = numel / 32;
+        const long long w2 = (n32 + threads - 1) / threads;
+        const int b2 = (int)(w2 < (long long)sm_count * 16 ? w2 : (long long)sm_count * 16);
+        if (out_dt == RT_F16) return launch_pdl(dequant_q4g_kernel<__half>, dim3(b2), dim3(threads), 0, stream, codes, s16, zeros, (__half *)dst, n32, shift);
+        return launch_pdl(dequant_q4g_kernel<float>, dim3(b2), dim3(threads), 0, stream, codes, s16, zeros, (float *)dst, n32, shift);
     } else {
         return cudaErrorInvalidValue;
     }

@@ -148,4 +148,8 @@ cudaError_t launch_silu_mul(const void *full, void *out, long long rows, int ff,
 cudaError_t launch_transpose(const void *src, void *dst, int stacks, int rows, int cols, int dst_ld, int elem_size, cudaStream_t stream);
 cudaError_t launch_pad_rows16(const void *src, void *dst, long long rows, int k, int k_pad, int sm_count, cudaStream_t stream);
 
+// The operators around the Linears (residual_norm.cu, log_probs.cu): one launch each, descriptions already checked, rows > 0.
+cudaError_t launch_residual_norm(const rt_residual_norm &op, int sm_count, cudaStream_t stream);
+cudaError_t launch_log_probs(const rt_log_probs &op, int sm_count, cudaStream_t stream);
+
 } // namespace rt

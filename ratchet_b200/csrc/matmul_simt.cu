@@ -46,7 +46,8 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(MatmulParams p) {
             const int m = m0 + ml, k = k0 + kl;
             float v = 0.f;
             if (m < p.M && k < p.K)
-                v = lhs_element<KIND>(p.lhs, p.lhs_scales, abase + (p.trans_lhs ? (long long)k * p.M + m : (long long)m * p.K + k));
+                v = lhs_element<KIND>(p.lhs, p.lhs_scales, abase + (p.trans_lhs ? (long long)k * p.M + m : (long long)m * p.K + k),
+                                      p.lhs_zeros, p.lhs_group_shift);
             As[kl][ml] = v;
         }
 #pragma unroll
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(256) gemv_simt_kernel(MatmulParams p) {
         for (int k = lane; k < p.K; k += 32) {
             const float xk = to_f32(x[k]);
 #pragma unroll
-            for (int r = 0; r < GEMV_ROWS; r++) acc[r] = fmaf(lhs_element<KIND>(p.lhs, p.lhs_scales, abase[r] + k), xk, acc[r]);
+            for (int r = 0; r < GEMV_ROWS; r++) acc[r] = fmaf(lhs_element<KIND>(p.lhs, p.lhs_scales, abase[r] + k, p.lhs_zeros, p.lhs_group_shift), xk, acc[r]);
         }
     }
 #pragma unroll
@@ -353,6 +354,9 @@ cudaError_t launch_matmul_simt(const MatmulParams &p, rt_dtype lhs_dt, rt_dtype 
     case RT_Q8_0H: return launch_kind<LK_Q8H>(p, act_dt, gemv, stream);
     case RT_Q8_0F: return launch_kind<LK_Q8F>(p, act_dt, gemv, stream);
     case RT_Q4_K: return launch_kind<LK_Q4K>(p, act_dt, gemv, stream);
+    case RT_Q4_G32:
+    case RT_Q4_G64:
+    case RT_Q4_G128: return launch_kind<LK_Q4G>(p, act_dt, gemv, stream);
     default: return cudaErrorInvalidValue;
     }
 }

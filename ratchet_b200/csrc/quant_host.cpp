@@ -1,8 +1,9 @@
-// Host-side block formats: layouts, Q8_0 quantiser / dequantiser, GGUF transcode, Q4_K codec.
+// Host-side block formats: layouts, Q8_0 quantiser / dequantiser, GGUF transcode, Q4_K and 4-bit group codecs.
 // Restates crates/ratchet-core/src/quant.rs:26-124, crates/ratchet-core/src/dtype/blocks.rs:61-74,
 // crates/ratchet-core/src/gpu/align.rs:23-40 and crates/ratchet-loader/src/gguf/dtype.rs:44-110.
 // In the reference these run on the CPU as well (weights are quantised / transcoded on the host
 // and uploaded once), so this is the product's host code, not a fallback for a device kernel.
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 
@@ -29,6 +30,18 @@ Status dtype_segments(rt_dtype dt, uint64_t numel, rt_segment *segs, int *n) {
         segs[0] = {0, numel / 256 * 144};
         *n = 1;
         return Status::Ok();
+    case RT_Q4_G32:
+    case RT_Q4_G64:
+    case RT_Q4_G128: {
+        const uint64_t group = (uint64_t)q4_group(dt);
+        if (numel % group != 0)
+            return Status::Err(RT_ERR_SHAPE, std::string(dtype_name(dt)) + " tensors hold a multiple of " + std::to_string(group) + " values");
+        segs[0] = {0, align_up(numel / 2, 256)};
+        segs[1] = {segs[0].size, align_up(numel / group * 2, 256)};
+        segs[2] = {segs[1].offset + segs[1].size, align_up(numel / group, 256)};
+        *n = 3;
+        return Status::Ok();
+    }
     default: {
         uint64_t bytes = numel * dtype_size(dt);
         if (bytes < 16) bytes = 16;                           // MIN_STORAGE_BUFFER_SIZE (dtype/mod.rs:90)
@@ -49,7 +62,7 @@ static inline int32_t f32_as_i32(float v) {
 
 // quant.rs:26-79
 Status quantize_q8_0(const float *x, uint64_t numel, rt_dtype dt, uint8_t *out) {
-    rt_segment seg[2];
+    rt_segment seg[RT_MAX_SEGMENTS];
     int n;
     Status st = dtype_segments(dt, numel, seg, &n);
     if (!st.ok()) return st;
@@ -80,7 +93,7 @@ Status quantize_q8_0(const float *x, uint64_t numel, rt_dtype dt, uint8_t *out) 
 
 // quant.rs:81-124; the f16 form is the shaders' f16(q) * d (gemm.rs:400-406).
 Status dequantize_q8_0(const uint8_t *src, uint64_t numel, rt_dtype dt, float *out) {
-    rt_segment seg[2];
+    rt_segment seg[RT_MAX_SEGMENTS];
     int n;
     Status st = dtype_segments(dt, numel, seg, &n);
     if (!st.ok()) return st;
@@ -102,7 +115,7 @@ Status dequantize_q8_0(const uint8_t *src, uint64_t numel, rt_dtype dt, float *o
 
 // gguf/dtype.rs:44-73 (f32 scales) and 80-109 (f16 scales)
 Status transcode_gguf_q8_0(const uint8_t *blocks, uint64_t n_blocks, rt_dtype dt, uint8_t *out) {
-    rt_segment seg[2];
+    rt_segment seg[RT_MAX_SEGMENTS];
     int n;
     Status st = dtype_segments(dt, n_blocks * 32, seg, &n);
     if (!st.ok()) return st;
@@ -210,6 +223,54 @@ Status quantize_q4_k(const float *x, uint64_t numel, uint8_t *out) {
                 qs[32 * (j / 2) + l] |= (uint8_t)((j & 1) ? (q << 4) : q);
             }
         }
+    }
+    return Status::Ok();
+}
+
+// 4-bit codes under an f16 scale and a zero point per group: value = (q - z) * s.
+Status quantize_q4_group(const float *x, uint64_t numel, rt_dtype dt, bool symmetric, uint8_t *out) {
+    rt_segment seg[RT_MAX_SEGMENTS];
+    int n;
+    Status st = dtype_segments(dt, numel, seg, &n);
+    if (!st.ok()) return st;
+    const uint64_t group = (uint64_t)q4_group(dt);
+    std::memset(out, 0, seg[2].offset + seg[2].size);
+    for (uint64_t g = 0; g < numel / group; g++) {
+        const float *v = x + g * group;
+        float lo = 0.f, hi = 0.f;
+        for (uint64_t i = 0; i < group; i++) {
+            if (v[i] < lo) lo = v[i];
+            if (v[i] > hi) hi = v[i];
+        }
+        lo = std::fmax(lo, -FLT_MAX);
+        hi = std::fmin(hi, FLT_MAX);
+        float s = symmetric ? std::fmax(-lo, hi) / 7.0f : hi / 15.0f - lo / 15.0f;
+        const uint16_t sh = f32_to_f16(s > 65504.f ? 65504.f : s);
+        s = f16_to_f32(sh);
+        auto steps = [&](float a) { return s > 0.f ? std::nearbyint((double)a / s) : 0.0; };
+        // the zero point by the range's own ratio: it stays inside the range where s had to be cut to f16's largest
+        const double z = symmetric ? 8.0 : hi > lo ? std::nearbyint(15.0 * -(double)lo / ((double)hi - (double)lo)) : 0.0;
+        std::memcpy(out + seg[1].offset + g * 2, &sh, 2);
+        out[seg[2].offset + g] = (uint8_t)z;
+        for (uint64_t i = 0; i < group; i++) {
+            const double q = std::isnan(v[i]) ? z : std::fmin(std::fmax(steps(v[i]) + z, 0.0), 15.0);
+            out[(g * group + i) / 2] |= (uint8_t)((unsigned)q << (i & 1 ? 4 : 0));
+        }
+    }
+    return Status::Ok();
+}
+
+Status dequantize_q4_group(const uint8_t *src, uint64_t numel, rt_dtype dt, float *out) {
+    rt_segment seg[RT_MAX_SEGMENTS];
+    int n;
+    Status st = dtype_segments(dt, numel, seg, &n);
+    if (!st.ok()) return st;
+    const uint64_t group = (uint64_t)q4_group(dt);
+    for (uint64_t i = 0; i < numel; i++) {
+        uint16_t sh;
+        std::memcpy(&sh, src + seg[1].offset + i / group * 2, 2);
+        const int q = src[i / 2] >> (i & 1 ? 4 : 0) & 15, z = src[seg[2].offset + i / group] & 31;
+        out[i] = (float)(q - z) * f16_to_f32(sh);
     }
     return Status::Ok();
 }

@@ -62,8 +62,9 @@ bool multi_broadcast(const Dims &a, const Dims &b, Dims *out) {
     return true;
 }
 
-bool dtype_valid(int dt) { return dt >= RT_F32 && dt <= RT_Q4_K; }
-bool is_quantized(rt_dtype dt) { return dt == RT_Q8_0H || dt == RT_Q8_0F || dt == RT_Q4_K; }
+bool dtype_valid(int dt) { return dt >= RT_F32 && dt <= RT_Q4_G128; }
+bool is_quantized(rt_dtype dt) { return dt == RT_Q8_0H || dt == RT_Q8_0F || dt == RT_Q4_K || q4_group(dt) != 0; }
+int q4_group(rt_dtype dt) { return dt == RT_Q4_G32 ? 32 : dt == RT_Q4_G64 ? 64 : dt == RT_Q4_G128 ? 128 : 0; }
 
 const char *dtype_name(rt_dtype dt) {
     switch (dt) {
@@ -75,6 +76,9 @@ const char *dtype_name(rt_dtype dt) {
     case RT_Q8_0H: return "Q8_0H";
     case RT_Q8_0F: return "Q8_0F";
     case RT_Q4_K: return "Q4_K";
+    case RT_Q4_G32: return "Q4_G32";
+    case RT_Q4_G64: return "Q4_G64";
+    case RT_Q4_G128: return "Q4_G128";
     }
     return "?";
 }
@@ -92,6 +96,7 @@ rt_dtype activation_dt(rt_dtype dt) {
     case RT_Q8_0H: return RT_F16;
     case RT_Q8_0F: return RT_F32;
     case RT_Q4_K: return RT_F16;
+    case RT_Q4_G32: case RT_Q4_G64: case RT_Q4_G128: return RT_F16;
     default: return dt;
     }
 }
@@ -144,13 +149,15 @@ Status compute_c_shape(const Dims &a, const Dims &b, bool tl, bool tr, bool to, 
 }
 
 // OpGuards::check_dtypes (ops/matmul.rs:454-477).  The first four pairs are the reference's;
-// the others are this library's extensions (bf16 activations, Q4_K weights, f32-scaled Q8_0
+// the others are this library's extensions (bf16 activations, 4-bit weights, f32-scaled Q8_0
 // with f16 activations).
 static bool pair_allowed(rt_dtype l, rt_dtype r) {
     static const rt_dtype pairs[][2] = {
         {RT_F32, RT_F32}, {RT_F16, RT_F16}, {RT_Q8_0F, RT_F32}, {RT_Q8_0H, RT_F16},
         {RT_BF16, RT_BF16}, {RT_Q8_0H, RT_BF16}, {RT_Q4_K, RT_F16}, {RT_Q4_K, RT_BF16},
         {RT_Q8_0F, RT_F16},
+        {RT_Q4_G32, RT_F16}, {RT_Q4_G64, RT_F16}, {RT_Q4_G128, RT_F16},
+        {RT_Q4_G32, RT_BF16}, {RT_Q4_G64, RT_BF16}, {RT_Q4_G128, RT_BF16},
     };
     for (auto &p : pairs)
         if (p[0] == l && p[1] == r) return true;
@@ -253,6 +260,8 @@ Status resolve_spec(const rt_matmul_desc &d, Spec *s) {
         return Status::Err(RT_ERR_SHAPE, "Q8_0 needs the inner dimension to be a multiple of 32");
     if (d.lhs_dt == RT_Q4_K && s->K % 256 != 0)
         return Status::Err(RT_ERR_SHAPE, "Q4_K needs the inner dimension to be a multiple of 256");
+    if (const int group = q4_group(d.lhs_dt); group != 0 && s->K % group != 0)
+        return Status::Err(RT_ERR_SHAPE, std::string(dtype_name(d.lhs_dt)) + " needs the inner dimension to be a multiple of " + std::to_string(group));
     // MatmulMeta holds i32 extents (ops/matmul.rs:375-387)
     for (int64_t v : {s->M, s->N, s->K, s->stacks})
         if (v >= (int64_t(1) << 31)) return Status::Err(RT_ERR_SHAPE, "extent exceeds i32");

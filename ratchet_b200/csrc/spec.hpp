@@ -40,9 +40,11 @@ bool multi_broadcast(const Dims &a, const Dims &b, Dims *out);
 
 bool dtype_valid(int dt);
 bool is_quantized(rt_dtype dt);
+// values per group of a 4-bit group format (RT_Q4_G*), 0 for every other dtype
+int q4_group(rt_dtype dt);
 const char *dtype_name(rt_dtype dt);
 size_t dtype_size(rt_dtype dt);
-// activation dtype of a weight dtype (dtype/mod.rs:77-83); Q4_K pairs with f16.
+// activation dtype of a weight dtype (dtype/mod.rs:77-83); the 4-bit formats pair with f16.
 rt_dtype activation_dt(rt_dtype dt);
 
 // The resolved node: everything a kernel launch needs to know about the problem.
@@ -58,6 +60,8 @@ struct Spec {
     int64_t bias_len = 0;
     int epilogue = 0;
 };
+
+Status dtype_segments(rt_dtype dt, uint64_t numel, rt_segment *segs, int *n); // at most RT_MAX_SEGMENTS
 
 Status compute_c_shape(const Dims &a, const Dims &b, bool trans_lhs, bool trans_rhs, bool trans_out, Dims *out);
 Status resolve_spec(const rt_matmul_desc &desc, Spec *spec);

@@ -37,6 +37,9 @@ class DType(enum.IntEnum):
     Q8_0H = _lib.RT_Q8_0H
     Q8_0F = _lib.RT_Q8_0F
     Q4_K = _lib.RT_Q4_K
+    Q4_G32 = _lib.RT_Q4_G32
+    Q4_G64 = _lib.RT_Q4_G64
+    Q4_G128 = _lib.RT_Q4_G128
 
     def size_of(self) -> int:
         return int(_lib.load().rt_dtype_size(int(self)))
@@ -249,19 +252,40 @@ class Executable:
     def __init__(self, device: Device, nodes: Sequence["Tensor"], use_graph: bool = True):
         self.device = device
         self._keep = list(nodes)
-        arr = (_lib.rt_dispatch * len(nodes))()
-        for i, t in enumerate(nodes):
-            if t.op is None or not isinstance(t.storage, GpuBuffer):
-                raise RatchetError(_lib.RT_ERR_ARG, "RT_ERR_ARG", "Executable nodes must be resolved op outputs")
-            arr[i].plan = device.plan_for(t.op.desc)
-            arr[i].lhs, arr[i].rhs = t.op.lhs.ptr, t.op.rhs.ptr
-            arr[i].bias = t.op.bias.ptr if t.op.bias is not None else None
-            arr[i].out = t.ptr
-            arr[i].opts.flags = _lib.RT_LAUNCH_LHS_CONSTANT if t.op.lhs.op is None else 0
         self._h = c_void_p()
-        check(_lib.load().rt_executable_create(device._h, arr, len(nodes), int(use_graph), byref(self._h)))
+        if all(t.op is None or isinstance(t.op, Matmul) for t in nodes):
+            arr = (_lib.rt_dispatch * len(nodes))()
+            for i, t in enumerate(nodes):
+                self._bind(arr[i], t)
+            check(_lib.load().rt_executable_create(device._h, arr, len(nodes), int(use_graph), byref(self._h)))
+        else:
+            # an operator with several outputs is one step, where the first of them is listed
+            first = {id(t.op): t for t in reversed(nodes)}
+            nodes = [t for t in nodes if first[id(t.op)] is t]
+            steps = (_lib.rt_step * len(nodes))()
+            for step, t in zip(steps, nodes):
+                if isinstance(t.op, Matmul):
+                    step.kind = _lib.RT_STEP_MATMUL
+                    self._bind(step.matmul, t)
+                else:
+                    self._resolved(t)
+                    t.op.bind(step)
+            check(_lib.load().rt_executable_create_steps(device._h, steps, len(nodes), int(use_graph), byref(self._h)))
         self.launches = int(_lib.load().rt_executable_launches(self._h))
         self.kernel = _lib.load().rt_executable_kernel(self._h).decode()
+
+    @staticmethod
+    def _resolved(t: "Tensor") -> None:
+        if t.op is None or not isinstance(t.storage, GpuBuffer):
+            raise RatchetError(_lib.RT_ERR_ARG, "RT_ERR_ARG", "Executable nodes must be resolved op outputs")
+
+    def _bind(self, d: "_lib.rt_dispatch", t: "Tensor") -> None:
+        self._resolved(t)
+        d.plan = self.device.plan_for(t.op.desc)
+        d.lhs, d.rhs = t.op.lhs.ptr, t.op.rhs.ptr
+        d.bias = t.op.bias.ptr if t.op.bias is not None else None
+        d.out = t.ptr
+        d.opts.flags = _lib.RT_LAUNCH_LHS_CONSTANT if t.op.lhs.op is None else 0
 
     @classmethod
     def _adopt(cls, device: Device, handle: c_void_p, keep) -> "Executable":
@@ -361,8 +385,45 @@ class Matmul:
         return [self.lhs, self.rhs] + ([self.bias] if self.bias is not None else [])
 
 
+class LazyOp:
+    """A node of the graph that is not a Matmul: one launch with one or more outputs.  A subclass names its operands (`srcs`),
+    the shapes and dtypes of what it writes (`specs`) and how a launch is described (`bind`, which fills an rt_step)."""
+
+    specs: Sequence = ()
+    _buffers: Optional[list] = None  # one per output, once launched
+
+    def outputs(self, device: Device) -> "list[Tensor]":
+        outs = [Tensor(shape, dt, device, None, self) for shape, dt in self.specs]
+        for i, t in enumerate(outs):
+            t._output = i
+        return outs
+
+    def srcs(self) -> "list[Tensor]":
+        raise NotImplementedError
+
+    def bind(self, step: "_lib.rt_step") -> None:
+        raise NotImplementedError
+
+    def launch(self, device: Device) -> None:
+        """Enqueues the operator on the device's stream, its outputs in new buffers."""
+        self._buffers = [GpuBuffer(device, dt.nbytes(math.prod(shape))) for shape, dt in self.specs]
+        step = _lib.rt_step()
+        try:
+            self.bind(step)
+            lib = _lib.load()
+            if step.kind == _lib.RT_STEP_RESIDUAL_NORM:
+                check(lib.rt_residual_norm_launch(device._h, byref(step.norm), None))
+            else:
+                check(lib.rt_log_probs_launch(device._h, byref(step.log_probs), None))
+        except Exception:
+            self._buffers = None
+            raise
+
+
 class Tensor:
     """An immutable, possibly lazy tensor (tensor.rs:40-133)."""
+
+    _output = 0  # which output of its op (a Matmul has one)
 
     def __init__(self, shape: Sequence[int], dt: DType, device: Device, storage=None, op: Optional[Matmul] = None):
         self.shape = [int(s) for s in shape]
@@ -459,6 +520,9 @@ class Tensor:
                 order.append(t)
                 continue
             stack += (t, None)
+            if isinstance(op, LazyOp):
+                stack += reversed(op.srcs())
+                continue
             if op.bias is not None:
                 stack.append(op.bias)
             stack += (op.rhs, op.lhs)
@@ -467,8 +531,40 @@ class Tensor:
     def resolve(self, sync: bool = True) -> "Tensor":
         """Tensor::resolve (tensor.rs:738-787): plan + dispatch every unresolved node, then wait."""
         device = self.device.try_gpu()
-        lib = _lib.load()
         todo = [t for t in self.execution_order() if t.storage is None]
+        if any(isinstance(t.op, LazyOp) for t in todo):
+            self._resolve_mixed(device, todo)
+        else:
+            self._resolve_matmuls(device, todo)
+        if sync:
+            device.sync()
+        return self
+
+    @staticmethod
+    def _resolve_mixed(device: Device, todo: "list[Tensor]") -> None:
+        """Runs of Matmul nodes in one native call each, the other operators between them."""
+        inside = {id(t) for t in todo}
+        for t in todo:
+            if t.op is None:
+                raise RatchetError(_lib.RT_ERR_ARG, "RT_ERR_ARG", "unresolved tensor without an op")
+            for s in t.op.srcs():
+                if id(s) not in inside and not (isinstance(s.storage, GpuBuffer) and s.device is device):
+                    raise RatchetError(_lib.RT_ERR_ARG, "RT_ERR_ARG", f"TensorError: operand on {s.device}, expected {device}")
+        run: "list[Tensor]" = []
+        for t in todo:
+            if not isinstance(t.op, LazyOp):
+                run.append(t)
+                continue
+            Tensor._resolve_matmuls(device, run)
+            run = []
+            if t.op._buffers is None:
+                t.op.launch(device)
+            t.storage = t.op._buffers[t._output]
+        Tensor._resolve_matmuls(device, run)
+
+    @staticmethod
+    def _resolve_matmuls(device: Device, todo: "list[Tensor]") -> None:
+        lib = _lib.load()
         if todo:
             position = {id(t): i for i, t in enumerate(todo)}
             stamp = lib.rt_routing_stamp()
@@ -497,9 +593,12 @@ class Tensor:
                 b.device, b._h, b.ptr, b.size = device, outs[3 * i], outs[3 * i + 1], outs[3 * i + 2]
                 t.storage = b
             check(status)
-        if sync:
-            device.sync()
-        return self
+
+    def log_probs(self, tokens: "Optional[Tensor]" = None, top: int = 0):
+        """Of logits [.., vocab]: each row's given token's log probability, the row's entropy and its `top` likeliest tokens
+        (a `LogProbs` of lazy tensors, see `ops.py`)."""
+        from .ops import log_probs
+        return log_probs(self, tokens, top)
 
     def to(self, device: Device, out: Optional[np.ndarray] = None) -> "Tensor":
         """Tensor::to (tensor.rs:864-870).  GPU->CPU may write into `out` (e.g. a pinned array)."""
@@ -608,12 +707,24 @@ class Quantizer:
         return Tensor(tensor.shape, DType.Q4_K, Device.CPU, out)
 
     @staticmethod
+    def q4_group_quantize(tensor: Tensor, dt: DType = DType.Q4_G128, symmetric: bool = False) -> Tensor:
+        """f32 CPU tensor -> 4-bit codes with an f16 scale and a zero point per group of 32, 64 or 128 values of a row."""
+        if tensor.dt != DType.F32 or tensor.device.is_gpu():
+            raise InvariantError(_lib.RT_ERR_INVARIANT, "RT_ERR_INVARIANT", "q4_group_quantize needs an f32 CPU tensor")
+        x = np.ascontiguousarray(tensor.to_numpy().reshape(-1))
+        out = np.empty(DType(dt).nbytes(x.size), dtype=np.uint8)
+        check(_lib.load().rt_quantize_q4_group(x.ctypes.data_as(c_void_p), x.size, int(dt), int(symmetric), out.ctypes.data_as(c_void_p)))
+        return Tensor(tensor.shape, dt, Device.CPU, out)
+
+    @staticmethod
     def dequantize_bytes(raw: np.ndarray, dt: DType, numel: int) -> np.ndarray:
         raw = np.ascontiguousarray(raw, dtype=np.uint8)
         out = np.empty(numel, dtype=np.float32)
         lib = _lib.load()
         if dt == DType.Q4_K:
             check(lib.rt_dequantize_q4_k(raw.ctypes.data_as(c_void_p), numel, out.ctypes.data_as(c_void_p)))
+        elif dt in (DType.Q4_G32, DType.Q4_G64, DType.Q4_G128):
+            check(lib.rt_dequantize_q4_group(raw.ctypes.data_as(c_void_p), numel, int(dt), out.ctypes.data_as(c_void_p)))
         else:
             check(lib.rt_dequantize_q8_0(raw.ctypes.data_as(c_void_p), numel, int(dt), out.ctypes.data_as(c_void_p)))
         return out
