@@ -71,7 +71,7 @@ struct rt_buffer {
     uint64_t klass = 0; // bytes allocated
 };
 
-enum PlanKernel { PK_GEMM_SIMT, PK_GEMV_SIMT, PK_Q8F_GEMV, PK_Q4K_GEMV_F16, PK_ROWVEC_MAT, PK_Q8_GEMV_MMA, PK_Q8_GEMV_UMMA, PK_Q4K_GEMV, PK_Q4K_GEMV_UMMA, PK_GEMM_UMMA };
+enum PlanKernel { PK_GEMM_SIMT, PK_GEMV_SIMT, PK_Q8F_GEMV, PK_Q4K_GEMV_F16, PK_ROWVEC_MAT, PK_Q8_GEMV_MMA, PK_Q8_GEMV_UMMA, PK_Q4K_GEMV, PK_Q4K_GEMV_UMMA, PK_Q4_GROUP_GEMV, PK_GEMM_UMMA };
 
 struct rt_plan {
     rt_device *dev = nullptr;
@@ -83,6 +83,8 @@ struct rt_plan {
     int nv = 1;
     GemvUmmaConfig gemv_umma{};
     Q4kUmmaConfig q4k_umma{};
+    Q4GroupConfig q4_group{};
+    int q4_batches = 1;    // 4-bit group GEMV: batches that are not flattened into vectors
     int nv2 = 0;           // streaming Q8_0 kernel: vectors beyond the first launch's 8, taken 8 at a time (9..24 in all)
     bool chain_ok = false; // a Q8_0H x f16 GEMV the persistent chain kernel can take as a node
     MatmulParams params{}; // everything but the pointers
@@ -740,6 +742,8 @@ static rt_status build_plan(rt_device *dev, const rt_matmul_desc *desc, rt_plan 
     const bool short_rows = q8 && s.N == 1 && s.K <= 512 && s.M >= 16384 && s.K % 32 == 0;
     // the warp-MMA Q4_K kernel's launch shape for one vector (0: rows too long for its shared memory)
     const int q4k_one = desc->lhs_dt == RT_Q4_K && s.N == 1 && !empty ? q4k_gemv_pick_split(p.M, p.K, 1, (int)s.stacks, dev->sm_count) : 0;
+    // a batch against one 4-bit group weight is that many vectors: rhs rows and output rows both lie one behind the other
+    const bool q4_flat = q4_group(desc->lhs_dt) != 0 && s.lhs_stack == 1 && (s.trans_out || s.N == 1);
     if (gemv_split > 0 && !short_rows && desc->rhs_dt == RT_F16 && !s.trans_lhs && s.N >= 1 && s.N <= 8 && (s.N == 1 || s.trans_rhs) && s.K > 0 && !empty) {
         pl->nv = (int)s.N;
         pl->split = gemv_split;
@@ -807,6 +811,16 @@ static rt_status build_plan(rt_device *dev, const rt_matmul_desc *desc, rt_plan 
         pl->name = std::string("q4k_gemv_mma_nv") + std::to_string(pl->nv) + "_split" + std::to_string(pl->split & 0xff) +
                    (((pl->split >> 8) & 0xff) > 1 ? "_walk" + std::to_string((pl->split >> 8) & 0xff) + "x" + std::to_string((pl->split >> 16) & 0xff) + "buf"
                                                    : std::string());
+    } else if (q4_group(desc->lhs_dt) != 0 && !force_simt() && !empty && s.K > 0 && (s.N == 1 || s.trans_rhs) &&
+               (q4_flat ? s.stacks * s.N : s.N) <= Q4_GROUP_MAX_NV && (q4_flat || s.stacks <= 65535) &&
+               q4_group_gemv_config(p.M, p.K, q4_group(desc->lhs_dt), (int)(q4_flat ? s.stacks * s.N : s.N), (int)(q4_flat ? 1 : s.stacks),
+                                    s.epilogue == RT_EPILOGUE_SILU_MUL, dev->sm_count, &pl->q4_group)) {
+        pl->kernel = PK_Q4_GROUP_GEMV;
+        pl->nv = (int)(q4_flat ? s.stacks * s.N : s.N);
+        pl->q4_batches = (int)(q4_flat ? 1 : s.stacks);
+        if (q4_flat) p.trans_out = 1; // (one column is the same memory either way)
+        pl->name = std::string("q4_group_gemv_g") + std::to_string(q4_group(desc->lhs_dt)) + "_nv" + std::to_string(pl->nv) + "_k" +
+                   std::to_string(pl->q4_group.parts) + "x" + std::to_string(pl->q4_group.ranks) + "_rows" + std::to_string(pl->q4_group.rows);
     } else if (s.M == 1 && s.N >= 2 && !s.trans_lhs && !s.trans_rhs && desc->lhs_dt == desc->rhs_dt && !is_quantized(desc->lhs_dt) &&
                (desc->rhs_dt == RT_F32 || desc->rhs_dt == RT_F16 || desc->rhs_dt == RT_BF16) && !empty && !force_simt() &&
                s.stacks <= 65535) {
@@ -942,7 +956,7 @@ static rt_status build_plan(rt_device *dev, const rt_matmul_desc *desc, rt_plan 
         pl->name = std::string("gemm_simt_") + dtype_name(desc->lhs_dt) + "_" + dtype_name(desc->rhs_dt);
     }
     if (s.epilogue == RT_EPILOGUE_SILU_MUL) {
-        if (pl->kernel == PK_Q4K_GEMV_F16) {
+        if (pl->kernel == PK_Q4K_GEMV_F16 || pl->kernel == PK_Q4_GROUP_GEMV) {
             pl->name += "+silu_mul"; // a CTA holds gate rows and their up rows
         } else if (pl->kernel == PK_GEMM_UMMA && !pl->tf32x3) {
             pl->name += "_silu_mul_paired_tiles"; // gate and up rows of a column meet in one tile
@@ -1170,6 +1184,15 @@ static rt_status launch_node(rt_plan *plan, const void *lhs, const void *rhs, co
         if ((reinterpret_cast<uintptr_t>(lhs) | reinterpret_cast<uintptr_t>(rhs)) % 16 != 0)
             return fail(RT_ERR_ARG, "rt_matmul_launch: lhs and rhs must be 16-byte aligned");
         e = launch_q4k_gemv_umma(p, plan->nv, plan->q4k_umma, (flags & RT_LAUNCH_LHS_CONSTANT) != 0, st);
+        break;
+    case PK_Q4_GROUP_GEMV:
+        if ((reinterpret_cast<uintptr_t>(lhs) | reinterpret_cast<uintptr_t>(rhs)) % 16 != 0) { // it loads 16 bytes at a time
+            if (s.epilogue == RT_EPILOGUE_SILU_MUL) return fail(RT_ERR_ARG, "rt_matmul_launch: lhs and rhs must be 16-byte aligned");
+            e = launch_matmul_simt(p, s.desc.lhs_dt, s.desc.rhs_dt, s.N == 1, st);
+            break;
+        }
+        e = launch_q4_group_gemv(p, s.desc.rhs_dt, plan->nv, plan->q4_batches, plan->q4_group, s.epilogue == RT_EPILOGUE_SILU_MUL,
+                                 (flags & RT_LAUNCH_LHS_CONSTANT) != 0, st);
         break;
     case PK_Q8_GEMV_UMMA:
         if ((reinterpret_cast<uintptr_t>(lhs) | reinterpret_cast<uintptr_t>(rhs)) % 16 != 0)

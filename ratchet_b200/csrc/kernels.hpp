@@ -100,6 +100,19 @@ bool q4k_gemv_umma_config(int M, int K, int nv, int sm_count, Q4kUmmaConfig *cfg
 cudaError_t launch_q4k_gemv_umma(const MatmulParams &p, int nv, const Q4kUmmaConfig &cfg, bool lhs_constant, cudaStream_t stream);
 cudaError_t gemv_q4k_umma_bind_wait_error(int *word);
 
+// 4-bit group weights x f16 / bf16, 1..16 vectors (rhs stored [nv][K]), K a multiple of the group, lhs and rhs 16-byte aligned;
+// pair: lhs rows are gate | up, the output their fold.  A batch with a vector set of its own per weight or per launch is `batches`.
+struct Q4GroupConfig {
+    int units, parts, ranks; // 16-row tiles of a CTA, warps of a tile and CTAs of a cluster along K
+    int rows, per_rank, per_part, stride, nvs;
+    uint32_t xsum_at, up_at, scales_at, part_at;
+    size_t smem_bytes;
+};
+constexpr int Q4_GROUP_MAX_NV = 16;
+bool q4_group_gemv_config(int M, int K, int group, int nv, int batches, bool pair, int sm_count, Q4GroupConfig *out); // false: K too long
+cudaError_t launch_q4_group_gemv(const MatmulParams &p, rt_dtype act, int nv, int batches, const Q4GroupConfig &c, bool pair, bool lhs_constant,
+                                 cudaStream_t stream);
+
 // Dense f32 GEMM on the tensor cores, three TF32 MMAs per product (f32-class accuracy): D[R][S] = P[R][K] . Q[S][K]^T.
 bool umma_tf32_supported(long long K);
 int umma_tf32_pick_bn(int R, int S, int stacks, int sm_count);
