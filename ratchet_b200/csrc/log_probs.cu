@@ -9,24 +9,24 @@
 //    top-th largest of all threads' largest, and are no smaller themselves: a bound for that from the warps' largest few, then only
 //    those threads read their chunks again (from L2) and collect what reaches it, a few more values than asked for.  Each counts
 //    how many are larger, which is its place.  Rows with more ties than the collection holds take the values one by one.
-//  * What is not finite: -inf adds nothing (t is held at -2000, a power of zero).  A row that has a NaN or +inf is known by its
-//    largest value.  A row of nothing but -inf, or of values whose t overflows (f32's and bf16's lowest), has S = 0.
+//  * What is not finite: -inf counts as the type's lowest or -1e38, a power of zero.  A row that has a NaN or +inf is known by its
+//    largest value.  A row of nothing but -inf, or of values below -1e38 (f32's and bf16's lowest as a mask), has S = 0.
 #include <algorithm>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "kernels.hpp"
 
 namespace rt {
 
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
-constexpr int UNROLL = 4;          // chunks a thread has in flight
-constexpr int LIST = 64;           // thread maxima that the bound is taken from
-constexpr int MOST = THREADS;      // values collected
+constexpr int GROUP = 2, GROUPS = 4; // chunks a thread asks for and works on together, and how many such groups are on their way
+constexpr int LIST = 64;             // thread maxima that the bound is taken from, at most
+constexpr int MOST = 512;          // values collected
 constexpr int MAX_RANKS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float NO_REFERENCE = -1e38f, LOW = -2000.f;
+constexpr float NO_REFERENCE = -1e38f, LOWEST = -1e38f; // values below LOWEST count as it: their t is finite and 2^t is 0
 using Order = unsigned long long;
 
 // larger value = larger word; -0 counts as +0, NaN as the largest; 0 is no value's word
@@ -51,19 +51,22 @@ __device__ __forceinline__ float exp2_approx(float t) {
     return d;
 }
 
-// A chunk's values; 16-bit types take the largest (NaN if there is one) two at a time.
+// A chunk's values, and its largest (NaN if there is one): `wide` words hold the places' largest so far, 16-bit types two places a
+// word.  raised() is the chunk with values below LOWEST (and NaN) lifted to about that.
 template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     static constexpr int N = 4;
+    static constexpr uint32_t MINUS_INF = 0xff800000u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
     }
-    static __device__ __forceinline__ float largest(const uint4 &r) {
-        return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)), max_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
-    }
+    static __device__ __forceinline__ uint32_t wider(uint32_t a, uint32_t b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ float widest(uint32_t a) { return __uint_as_float(a); }
+    static __device__ __forceinline__ uint32_t raised(uint32_t a) { return __float_as_uint(fmaxf(__uint_as_float(a), LOWEST)); }
 };
 template <> struct Chunk<__half> {
     static constexpr int N = 8;
+    static constexpr uint32_t MINUS_INF = 0xfc00fc00u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -72,28 +75,46 @@ template <> struct Chunk<__half> {
             v[2 * i] = f.x, v[2 * i + 1] = f.y;
         }
     }
-    static __device__ __forceinline__ float largest(const uint4 &r) {
-        const __half2 a = __hmax2_nan(*reinterpret_cast<const __half2 *>(&r.x), *reinterpret_cast<const __half2 *>(&r.y));
-        const __half2 b = __hmax2_nan(*reinterpret_cast<const __half2 *>(&r.z), *reinterpret_cast<const __half2 *>(&r.w));
-        const float2 f = __half22float2(__hmax2_nan(a, b));
+    static __device__ __forceinline__ uint32_t wider(uint32_t a, uint32_t b) {
+        return h2_as_u32(__hmax2_nan(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b)));
+    }
+    static __device__ __forceinline__ float widest(uint32_t a) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a));
         return max_nan(f.x, f.y);
+    }
+    static __device__ __forceinline__ uint32_t raised(uint32_t a) { // -65504
+        const uint32_t low = 0xfbfffbffu;
+        return h2_as_u32(__hmax2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&low)));
     }
 };
 template <> struct Chunk<__nv_bfloat16> {
     static constexpr int N = 8;
+    static constexpr uint32_t MINUS_INF = 0xff80ff80u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-    static __device__ __forceinline__ float largest(const uint4 &r) {
-        const __nv_bfloat162 a = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&r.x), *reinterpret_cast<const __nv_bfloat162 *>(&r.y));
-        const __nv_bfloat162 b = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&r.z), *reinterpret_cast<const __nv_bfloat162 *>(&r.w));
-        const __nv_bfloat162 m = __hmax2_nan(a, b);
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(&m);
-        return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    static __device__ __forceinline__ uint32_t as_word(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+    static __device__ __forceinline__ uint32_t wider(uint32_t a, uint32_t b) {
+        return as_word(__hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b)));
+    }
+    static __device__ __forceinline__ float widest(uint32_t a) { return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)); }
+    static __device__ __forceinline__ uint32_t raised(uint32_t a) { // -9.97e37
+        const uint32_t low = 0xfe96fe96u;
+        return as_word(__hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&low)));
     }
 };
+template <typename T> __device__ __forceinline__ uint32_t wide_of(const uint4 &r) {
+    return Chunk<T>::wider(Chunk<T>::wider(r.x, r.y), Chunk<T>::wider(r.z, r.w));
+}
+
+// 16 bytes from global to shared memory behind the thread's back, and the wait for all but the newest `GROUPS` groups of them
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int GROUPS> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(GROUPS) : "memory"); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -129,25 +150,63 @@ struct Sums {
     }
 };
 
-template <typename T> __global__ void __launch_bounds__(THREADS, 2) log_probs_kernel(const __grid_constant__ rt_log_probs p, int ranks) {
-    constexpr int N = Chunk<T>::N;
-    __shared__ float red[2][WARPS], meet[4]; // what the CTAs of a cluster tell: c, s, w of the slice
+// The values at and above `least` of a row's slice, one by one in falling order: for rows of many equal values, which the collection
+// does not hold.
+template <typename T, int TH, typename Each>
+__device__ __noinline__ void take_one_by_one(Each each, int vocab, int n, Order *top, Order *best_of) {
+    Order last = ~0ull;
+    auto next = [&]() { // this thread's largest below the last one taken
+        Order o = 0;
+        each([&](float f, long long id) {
+            if (id < 0 || id >= vocab) return;
+            const Order q = order_of(order_bits(f), (uint32_t)id);
+            if (q < last && q > o) o = q;
+        });
+        return o;
+    };
+    Order own = next();
+    for (int k = 0; k < n; k++) {
+        Order o = own;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const Order other = __shfl_xor_sync(0xffffffffu, o, d);
+            o = other > o ? other : o;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) best_of[threadIdx.x >> 5] = o;
+        __syncthreads();
+        o = best_of[0];
+        for (int d = 1; d < TH / 32; d++) o = best_of[d] > o ? best_of[d] : o;
+        if (threadIdx.x == 0) top[k] = o;
+        last = o;
+        if (own == o) own = next();
+    }
+}
+
+// TH threads; `ranks` CTAs of a cluster to a row
+template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 5 : 2) log_probs_kernel(const __grid_constant__ rt_log_probs p, int ranks) {
+    constexpr int N = Chunk<T>::N, WARPS = TH / 32;
+    __shared__ float3 sums_of[WARPS];
+    __shared__ float meet[3]; // what the CTAs of a cluster tell: c, s, w of the slice
     __shared__ uint32_t bits_of[WARPS], list[LIST], slice_bits, bound;
-    __shared__ int count;
-    __shared__ Order found[MOST], top[RT_LOG_PROBS_MAX_TOP], all[MAX_RANKS * RT_LOG_PROBS_MAX_TOP], best_of[WARPS];
+    __shared__ int count, marked, redo;
+    __shared__ short mark[TH];
+    extern __shared__ __align__(16) uint4 ring[]; // [GROUPS][GROUP][TH], a thread's own places: no barriers
+    __shared__ __align__(16) Order found[MOST], all[MAX_RANKS * RT_LOG_PROBS_MAX_TOP];
+    __shared__ Order top[RT_LOG_PROBS_MAX_TOP], best_of[WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = ranks > 1 ? (int)cluster_rank() : 0;
-    const long long row = blockIdx.x / ranks;
+    const long long row = ranks > 1 ? blockIdx.x / ranks : blockIdx.x;
     const int vocab = (int)p.vocab;
     const T *const v = (const T *)p.logits + row * p.ld;
     // chunks lie on 16-byte boundaries: chunk i has values i N - shift .. + N - 1 of the row; the first and the last may be partial
     const int shift = (int)(reinterpret_cast<uintptr_t>(v) % 16 / sizeof(T)), chunks = (int)(((long long)vocab + shift + N - 1) / N);
     const uint4 *const base = reinterpret_cast<const uint4 *>(v - shift);
-    const int per = (chunks + ranks - 1) / ranks, begin = min(chunks, rank * per), end = min(chunks, begin + per);
+    const int per = ranks > 1 ? (chunks + ranks - 1) / ranks : chunks, begin = min(chunks, rank * per), end = min(chunks, begin + per);
 
-    if (tid == 0) count = 0;
+    if (tid == 0) count = marked = 0, bound = 0xffffffffu;
     float token_value = 0.f;
     bool token_there = false;
     if (tid == 0 && rank == 0 && p.log_prob) {
@@ -157,8 +216,11 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) log_probs_ke
     }
 
     // ---- one pass: sums and the thread's largest value
-    auto partial = [&](int i) { return (i == 0 && shift > 0) || (i == chunks - 1 && (long long)chunks * N - shift > vocab); };
-    auto guarded = [&](int i) { // values outside the row as -inf
+    const bool partial0 = shift > 0, partial1 = (long long)chunks * N - shift > vocab;
+    const int first_whole = begin + (begin == 0 && begin < end && (partial0 || (chunks == 1 && partial1))), last_whole = end - (end > first_whole && end == chunks && partial1);
+    // the partial chunks: the first one is thread 0's, the last one thread 32's
+    const int odd = tid == 0 && first_whole > begin ? begin : tid == 32 && last_whole < end ? end - 1 : -1;
+    auto guarded = [=](int i) { // values outside the row as -inf
         T raw[N];
 #pragma unroll
         for (int k = 0; k < N; k++) {
@@ -169,160 +231,209 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) log_probs_ke
         memcpy(&r, raw, 16);
         return r;
     };
-    Sums sum{NO_REFERENCE, 0.f, 0.f};
-    float largest = -INFINITY;
-    bool any = false;
-    auto take = [&](const uint4 &r) {
-        const float m = Chunk<T>::largest(r);
-        largest = max_nan(largest, m);
+    // the largest values of the thread's best and second-best group of chunks (NaN above all), and where the best one begins
+    float c = NO_REFERENCE, best = -INFINITY, second = -INFINITY;
+    int best_at = 0;
+    unsigned long long s2 = 0, w2 = 0; // pairs of sums
+    const unsigned long long log2e2 = pack2f(LOG2E, LOG2E);
+    auto raise = [&](float m) { // the largest of what comes next
         const float mc = m * LOG2E;
-        if (mc > sum.c + 8.f) sum.move(mc);
-        float f[N];
-        Chunk<T>::values(r, f);
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            const float t = fmaxf(fmaf(f[k], LOG2E, -sum.c), LOW), e = exp2_approx(t);
-            sum.s += e;
-            sum.w = fmaf(e, t, sum.w);
+        if (mc > c + 8.f) {
+            Sums sum{c, sum2(s2), sum2(w2)};
+            sum.move(mc);
+            c = mc, s2 = pack2f(sum.s, 0.f), w2 = pack2f(sum.w, 0.f);
         }
     };
-    const int first_whole = begin + (begin < end && partial(begin)), last_whole = end - (end > first_whole && partial(end - 1));
-    int i = first_whole + tid;
-    for (; i + (UNROLL - 1) * THREADS < last_whole; i += UNROLL * THREADS) {
-        uint4 r[UNROLL];
+    auto add = [&](const uint4 &r) {
+        const unsigned long long minus_c = pack2f(-c, -c);
+        float f[N];
+        Chunk<T>::values(make_uint4(Chunk<T>::raised(r.x), Chunk<T>::raised(r.y), Chunk<T>::raised(r.z), Chunk<T>::raised(r.w)), f);
 #pragma unroll
-        for (int k = 0; k < UNROLL; k++) r[k] = __ldg(base + i + k * THREADS);
+        for (int k = 0; k < N; k += 2) {
+            const unsigned long long t = fma2(pack2f(f[k], f[k + 1]), log2e2, minus_c);
+            float t0, t1;
+            unpack2f(t, t0, t1);
+            const unsigned long long e = pack2f(exp2_approx(t0), exp2_approx(t1));
+            s2 = add2(s2, e);
+            w2 = fma2(e, t, w2);
+        }
+    };
+    const int mine_of = last_whole - first_whole - tid, my_chunks = mine_of > 0 ? (mine_of + TH - 1) / TH : 0;
+    const uint4 *from = base + first_whole + tid; // chunk k of the thread: from + k TH
+    uint4 *const place = ring + tid;
+    int asked = 0;
+    auto ask = [&](int part) {
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(place + part * GROUP * TH);
 #pragma unroll
-        for (int k = 0; k < UNROLL; k++) take(r[k]);
-        any = true;
+        for (int k = 0; k < GROUP; k++)
+            if (asked + k < my_chunks) copy_async(to + k * TH * 16, from + k * TH);
+        copy_commit();
+        asked += GROUP, from += GROUP * TH;
+    };
+#pragma unroll
+    for (int k = 0; k < GROUPS; k++) ask(k);
+    auto rank_group = [&](float m, int at) {
+        const bool first = !(m <= best);
+        second = first ? best : !(m <= second) ? m : second;
+        best = first ? m : best;
+        best_at = first ? at : best_at;
+    };
+    int left = my_chunks, part = 0;
+    for (; left >= GROUP; left -= GROUP, part = (part + 1) % GROUPS) {
+        copy_wait<GROUPS - 1>();
+        uint4 r[GROUP];
+#pragma unroll
+        for (int k = 0; k < GROUP; k++) r[k] = place[(part * GROUP + k) * TH];
+        uint32_t wide = wide_of<T>(r[0]);
+#pragma unroll
+        for (int k = 1; k < GROUP; k++) wide = Chunk<T>::wider(wide, wide_of<T>(r[k]));
+        const float m = Chunk<T>::widest(wide);
+        raise(m);
+        rank_group(m, my_chunks - left);
+        ask(part); // (into the places just read)
+#pragma unroll
+        for (int k = 0; k < GROUP; k++) add(r[k]);
     }
-    for (; i < last_whole; i += THREADS) take(__ldg(base + i)), any = true;
-    // the partial chunks: the first one is thread 0's, the last one thread 32's
-    const int odd = tid == 0 && first_whole > begin ? begin : tid == 32 && last_whole < end ? end - 1 : -1;
-    if (odd >= 0) take(guarded(odd)), any = true;
+    copy_wait<0>();
+    for (int k = 0; k < left; k++) {
+        const uint4 r = place[(part * GROUP + k) * TH];
+        const float m = Chunk<T>::widest(wide_of<T>(r));
+        raise(m);
+        rank_group(m, my_chunks - left + k);
+        add(r);
+    }
+    float odd_largest = -INFINITY;
+    if (odd >= 0) {
+        const uint4 r = guarded(odd);
+        odd_largest = Chunk<T>::widest(wide_of<T>(r));
+        raise(odd_largest);
+        add(r);
+    }
 
-    // ---- the CTA's sums and largest value
-    const uint32_t mine = any ? order_bits(largest) : 0u;
+    // ---- the warps' sums, and the list for the bound: the largest few thread maxima of each warp that has chunks
+    const uint32_t mine = my_chunks > 0 || odd >= 0 ? order_bits(max_nan(best, odd_largest)) : 0u;
     uint32_t warp_bits = __reduce_max_sync(0xffffffffu, mine);
-    float c = sum.c;
+    Sums sum{c, sum2(s2), sum2(w2)};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, o));
-    if (lane == 0) red[0][warp] = c, bits_of[warp] = warp_bits;
-    // the bound's list: the largest few thread maxima of each warp that has chunks
-    const int busy = min(WARPS, (last_whole - first_whole + 31) / 32 + 1), few = busy >= WARPS ? LIST / WARPS : min(32, LIST / busy);
-    const int listed = p.top ? min(LIST, busy * few) : 0;
-    if (p.top && warp < busy) {
-        uint32_t left = mine;
-        for (int k = 0; k < few; k++) {
-            if (k > 0) warp_bits = __reduce_max_sync(0xffffffffu, left);
-            const uint32_t who = __ballot_sync(0xffffffffu, left == warp_bits);
-            if (lane == __ffs(who) - 1) {
-                if (warp * few + k < LIST) list[warp * few + k] = left;
-                left = 0;
-            }
-        }
-    }
-    __syncthreads();
-    c = red[0][lane % WARPS];
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, o));
     sum.move(c);
-    float s = sum.s, w = sum.w;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), w += __shfl_xor_sync(0xffffffffu, w, o);
-    // (red[0] was read by all before it is written again: the shuffles above wait for the warp, the barrier for the CTA)
-    if (tid < listed) { // the top-th largest of the list; 0 where it is shorter
-        const uint32_t me = list[tid];
-        int above = 0;
-        for (int k = 0; k < listed; k++) above += list[k] > me || (list[k] == me && k < tid);
-        if (above == p.top - 1) bound = me;
-    }
-    if (tid == 0 && listed < p.top) bound = 0;
-    __syncthreads();
-    if (lane == 0) red[0][warp] = s, red[1][warp] = w;
-    if (p.top) {
-        const uint32_t least = max(bound, 1u);
-        if (mine >= least) { // this thread has values that may be among the largest
-            auto collect = [&](const uint4 &r, int at) {
-                float f[N];
-                Chunk<T>::values(r, f);
-#pragma unroll
-                for (int k = 0; k < N; k++) {
-                    const uint32_t b = order_bits(f[k]);
-                    const long long id = (long long)at * N - shift + k;
-                    if (b >= least && id >= 0 && id < vocab) {
-                        const int to = atomicAdd(&count, 1);
-                        if (to < MOST) found[to] = order_of(b, (uint32_t)id);
-                    }
-                }
-            };
-            int j = first_whole + tid;
-            for (; j + (UNROLL - 1) * THREADS < last_whole; j += UNROLL * THREADS) {
-                uint4 r[UNROLL];
-#pragma unroll
-                for (int k = 0; k < UNROLL; k++) r[k] = __ldg(base + j + k * THREADS);
-#pragma unroll
-                for (int k = 0; k < UNROLL; k++)
-                    if (order_bits(Chunk<T>::largest(r[k])) >= least) collect(r[k], j + k * THREADS);
-            }
-            for (; j < last_whole; j += THREADS) {
-                const uint4 r = __ldg(base + j);
-                if (order_bits(Chunk<T>::largest(r)) >= least) collect(r, j);
-            }
-            if (odd >= 0) collect(guarded(odd), odd);
+    for (int o = 16; o > 0; o >>= 1) sum.s += __shfl_xor_sync(0xffffffffu, sum.s, o), sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
+    if (lane == 0) sums_of[warp] = make_float3(c, sum.s, sum.w), bits_of[warp] = warp_bits;
+    const int busy = min(WARPS, (last_whole - first_whole + 31) / 32 + 1), few = min(32, (p.top * 3 / 2 + busy - 1) / busy), listed = busy * few; // (LIST at most)
+    if (warp < busy) {
+        uint32_t rest = mine;
+        for (int k = 0; k < few; k++) {
+            if (k > 0) warp_bits = __reduce_max_sync(0xffffffffu, rest);
+            const uint32_t who = __ballot_sync(0xffffffffu, rest == warp_bits);
+            if (lane == __ffs(who) - 1) list[warp * few + k] = rest, rest = 0;
         }
-        if (tid < p.top) top[tid] = 0;
     }
     __syncthreads();
-    s = red[0][lane % WARPS], w = red[1][lane % WARPS];
-    uint32_t bits = bits_of[lane % WARPS];
+
+    // ---- the slice's sums, in the first warp; the bound, by the next two
+    float s = 0.f, w = 0.f;
+    uint32_t bits = 0;
+    if (warp == 0) {
+        const float3 of = sums_of[lane % WARPS];
+        sum = Sums{of.x, of.y, of.z};
+        c = of.x;
+        bits = __reduce_max_sync(0xffffffffu, bits_of[lane % WARPS]);
 #pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), w += __shfl_xor_sync(0xffffffffu, w, o);
-    bits = __reduce_max_sync(0xffffffffu, bits);
+        for (int o = WARPS / 2; o > 0; o >>= 1) c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, o));
+        sum.move(c);
+        s = sum.s, w = sum.w;
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), w += __shfl_xor_sync(0xffffffffu, w, o);
+    }
     if (p.top) {
+        // the top-th largest of the list is the smallest that fewer than `top` are larger than; a list that is too short has none
+        if (tid >= 32 && tid - 32 < listed) {
+            const uint32_t me = list[tid - 32];
+            int above = listed < p.top ? p.top : 0;
+#pragma unroll 8
+            for (int k = 0; k < listed; k++) above += list[k] > me;
+            if (above < p.top) atomicMin(&bound, me);
+        }
+        if (tid == 0 && listed < p.top) bound = 0;
+        if (tid < p.top) top[tid] = 0;
+        __syncthreads();
+        const uint32_t least = max(bound, 1u);
+        auto push = [&](float f, int id) {
+            const uint32_t b = order_bits(f);
+            if (b >= least && (unsigned)id < (unsigned)vocab) {
+                const int to = atomicAdd(&count, 1);
+                if (to < MOST) found[to] = order_of(b, (uint32_t)id);
+            }
+        };
+        // A thread that has some of the largest looks at its best group again; where the second-best has some too, it is marked, and
+        // a warp goes over all of its chunks, a chunk a lane, and over a chunk that has some a value a lane.
+        if (mine >= least) {
+            if (order_bits(second) >= least) {
+                mark[atomicAdd(&marked, 1)] = (short)tid;
+            } else if (order_bits(best) >= least) {
+#pragma unroll
+                for (int g = 0; g < GROUP; g++) {
+                    if (best_at + g >= my_chunks) break;
+                    const int at = first_whole + tid + (best_at + g) * TH;
+                    const uint4 r = __ldg(base + at);
+                    float f[N];
+                    Chunk<T>::values(r, f);
+#pragma unroll
+                    for (int k = 0; k < N; k++) push(f[k], at * N - shift + k);
+                }
+            }
+            if (odd >= 0) {
+                float f[N];
+                Chunk<T>::values(guarded(odd), f);
+#pragma unroll
+                for (int k = 0; k < N; k++) push(f[k], odd * N - shift + k);
+            }
+        }
+        __syncthreads();
+        const int n_marked = marked;
+        for (int m = warp; m < n_marked; m += WARPS)
+            for (int at0 = first_whole + mark[m]; at0 < last_whole; at0 += 32 * TH) {
+                const int at = at0 + lane * TH;
+                uint4 r = make_uint4(0, 0, 0, 0);
+                bool has = false;
+                if (at < last_whole) {
+                    r = __ldg(base + at);
+                    has = order_bits(Chunk<T>::widest(wide_of<T>(r))) >= least;
+                }
+                for (uint32_t who = __ballot_sync(0xffffffffu, has); who; who &= who - 1) {
+                    const int src = __ffs(who) - 1;
+                    const uint4 u = make_uint4(__shfl_sync(0xffffffffu, r.x, src), __shfl_sync(0xffffffffu, r.y, src), __shfl_sync(0xffffffffu, r.z, src),
+                                               __shfl_sync(0xffffffffu, r.w, src));
+                    float f[N];
+                    Chunk<T>::values(u, f);
+                    float mine_of_it = f[0];
+#pragma unroll
+                    for (int k = 1; k < N; k++) mine_of_it = lane == k ? f[k] : mine_of_it;
+                    if (lane < N) push(mine_of_it, (at0 + src * TH) * N - shift + lane);
+                }
+            }
+        __syncthreads();
         const int n = count;
         if (n <= MOST) {
-            if (tid < n) {
-                const Order me = found[tid];
+            for (int e = tid; e < n; e += TH) {
+                const Order me = found[e];
                 int above = 0;
+#pragma unroll 4
                 for (int k = 0; k < n; k++) above += found[k] > me;
                 if (above < p.top) top[above] = me;
             }
-        } else { // many equal values: one after the other, each thread with its largest below the last one taken
-            Order last = ~0ull;
-            auto next = [&]() {
-                Order o = 0;
-                auto look = [&](const uint4 &r, int at) {
+        } else {
+            take_one_by_one<T, TH>([=](auto look) {
+                auto values = [=](const uint4 &r, int at) {
                     float f[N];
                     Chunk<T>::values(r, f);
-                    for (int k = 0; k < N; k++) {
-                        const long long id = (long long)at * N - shift + k;
-                        if (id < 0 || id >= vocab) continue;
-                        const Order q = order_of(order_bits(f[k]), (uint32_t)id);
-                        if (q < last && q > o) o = q;
-                    }
+                    for (int k = 0; k < N; k++) look(f[k], (long long)at * N - shift + k);
                 };
-                for (int j = first_whole + tid; j < last_whole; j += THREADS) look(__ldg(base + j), j);
-                if (odd >= 0) look(guarded(odd), odd);
-                return o;
-            };
-            Order own = next();
-            for (int k = 0; k < p.top; k++) {
-                Order o = own;
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) {
-                    const Order other = __shfl_xor_sync(0xffffffffu, o, d);
-                    o = other > o ? other : o;
-                }
-                __syncthreads();
-                if (lane == 0) best_of[warp] = o;
-                __syncthreads();
-                o = best_of[0];
-                for (int d = 1; d < WARPS; d++) o = best_of[d] > o ? best_of[d] : o;
-                if (tid == 0) top[k] = o;
-                last = o;
-                if (own == o) own = next();
-            }
+#pragma unroll 1
+                for (int at = first_whole + tid; at < last_whole; at += TH) values(__ldg(base + at), at);
+                if (odd >= 0) values(guarded(odd), odd);
+            }, vocab, p.top, top, best_of);
         }
     }
 
@@ -344,40 +455,41 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) log_probs_ke
             const int n = ranks * p.top;
             if (tid < n) all[tid] = load_peer(&top[tid % p.top], tid / p.top);
             __syncthreads();
-            if (tid < n) {
-                const Order me = all[tid];
-                int above = 0;
-                for (int k = 0; k < n; k++) above += all[k] > me || (all[k] == me && k < tid); // (slices without enough values have zeros)
-                if (above < p.top) top[above] = me; // (the peers read none of rank 0's after the barrier below; its own were read above)
-            }
+            const int e = tid >> 1; // two threads to a value
+            const Order me = e < n ? all[e] : 0;
+            int above = 0;
+#pragma unroll 4
+            for (int k = tid & 1; k < n; k += 2) above += all[k] > me || (all[k] == me && k < e); // (slices without enough values have zeros)
+            above += __shfl_xor_sync(0xffffffffu, above, 1);
+            if (e < n && above < p.top) top[above] = me; // (nobody else reads this CTA's any more)
         }
         cluster_sync(); // no CTA leaves while it may be read
         if (rank != 0) return;
     }
-    __syncthreads();
-
-    // ---- the row
+    // ---- the row, in the first warp, which has c, s, w and the largest value's bits
     bool nothing = bits <= MINUS_INF_BITS;
     const bool broken = bits >= INF_BITS; // +inf or NaN
-    if (!nothing && !broken && !(s > 0.f)) {
+    if (tid == 0) redo = !nothing && !broken && !(s > 0.f), slice_bits = bits;
+    __syncthreads();
+    if (redo) {
         // values whose t overflows: the lowest of f32 or bf16 and nothing above.  Differences to the largest are exact enough.
-        const float m = order_value(bits);
+        const float m = order_value(slice_bits);
         s = w = 0.f;
-        for (int j = tid; j < vocab; j += THREADS) {
-            const float t = fmaxf((to_f32(v[j]) - m) * LOG2E, LOW), e = exp2_approx(t);
+        for (int j = tid; j < vocab; j += TH) {
+            const float t = fmaxf((to_f32(v[j]) - m) * LOG2E, LOWEST), e = exp2_approx(t);
             s += e;
             w = fmaf(e, t, w);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), w += __shfl_xor_sync(0xffffffffu, w, o);
+        if (lane == 0) sums_of[warp] = make_float3(0.f, s, w);
         __syncthreads();
-        if (lane == 0) red[0][warp] = s, red[1][warp] = w;
-        __syncthreads();
-        s = red[0][lane % WARPS], w = red[1][lane % WARPS];
+        s = sums_of[lane % WARPS].y, w = sums_of[lane % WARPS].z;
 #pragma unroll
         for (int o = WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), w += __shfl_xor_sync(0xffffffffu, w, o);
         c = NAN; // the reference is m
     }
+    if (warp > 0) return;
     // differences to the largest value keep their bits, however far from zero the row lies
     const float log_s = log2f(s), m = order_value(bits), above = LN2 * (log_s - (c == c ? fmaf(m, LOG2E, -c) : 0.f)); // ln sum e^(v - m)
     auto log_prob = [&](float x) { return broken ? NAN : nothing ? -INFINITY : (x - m) - above; };
@@ -392,13 +504,15 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) log_probs_ke
     }
 }
 
-template <typename T> cudaError_t launch_t(const rt_log_probs &op, int sm_count, cudaStream_t stream) {
-    // few rows: a cluster to a row, as long as every thread of it gets a chunk
-    int ranks = 1;
-    while (ranks < MAX_RANKS && op.rows * ranks * 2 <= 2LL * sm_count && op.vocab / Chunk<T>::N >= 2LL * ranks * THREADS) ranks *= 2;
+template <typename T, int TH> cudaError_t launch_threads(const rt_log_probs &op, int ranks, cudaStream_t stream) {
+    constexpr size_t RING = GROUPS * GROUP * TH * sizeof(uint4);
+    static SmemAttr attr;
+    cudaError_t e = attr.ensure(log_probs_kernel<T, TH>, RING);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(op.rows * ranks));
-    lc.blockDim = dim3(THREADS);
+    lc.blockDim = dim3(TH);
+    lc.dynamicSmemBytes = RING;
     lc.stream = stream;
     cudaLaunchAttribute a[2];
     a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -408,7 +522,16 @@ template <typename T> cudaError_t launch_t(const rt_log_probs &op, int sm_count,
     a[1].val.clusterDim.y = a[1].val.clusterDim.z = 1;
     lc.attrs = a;
     lc.numAttrs = ranks > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&lc, log_probs_kernel<T>, op, ranks);
+    return cudaLaunchKernelEx(&lc, log_probs_kernel<T, TH>, op, ranks);
+}
+
+template <typename T> cudaError_t launch_t(const rt_log_probs &op, int sm_count, cudaStream_t stream) {
+    // Many rows: the work that a row costs beyond its values goes by its warps.  Few: more threads to a row, and a cluster's CTAs
+    // only where a thread would have more than 32 chunks, since two cluster barriers cost more than they save below that.
+    if (op.rows > 2LL * sm_count) return launch_threads<T, 256>(op, 1, stream);
+    int ranks = 1;
+    while (ranks < MAX_RANKS && op.rows * ranks * 2 <= 2LL * sm_count && op.vocab / Chunk<T>::N > 32LL * ranks * 512) ranks *= 2;
+    return launch_threads<T, 512>(op, ranks, stream);
 }
 
 } // namespace
