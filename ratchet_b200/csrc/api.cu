@@ -137,6 +137,7 @@ static const WaitFamily WAIT_FAMILIES[] = {
     {gemv_q4k_bind_wait_error, "a Q4_K GEMV", "its output is incomplete"},
     {gemv_q4k_umma_bind_wait_error, "a tensor-memory Q4_K GEMV", "its output is incomplete"},
     {gemv_bind_wait_error, "a GEMV", "its output is incomplete"},
+    {residual_norm_bind_wait_error, "a residual norm", "its outputs are incomplete"},
 };
 constexpr int N_WAIT_FAMILIES = (int)(sizeof(WAIT_FAMILIES) / sizeof(WAIT_FAMILIES[0]));
 constexpr int MAX_ORDINALS = 64;

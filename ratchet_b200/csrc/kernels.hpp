@@ -164,5 +164,6 @@ cudaError_t launch_pad_rows16(const void *src, void *dst, long long rows, int k,
 // The operators around the Linears (residual_norm.cu, log_probs.cu): one launch each, descriptions already checked, rows > 0.
 cudaError_t launch_residual_norm(const rt_residual_norm &op, int sm_count, cudaStream_t stream);
 cudaError_t launch_log_probs(const rt_log_probs &op, int sm_count, cudaStream_t stream);
+cudaError_t residual_norm_bind_wait_error(int *word);
 
 } // namespace rt

@@ -314,6 +314,78 @@ def test_norms_of_no_rows_and_of_many(gpu):
     assert np.all(close(got, normed(v.astype(np.float64), 0 * v.astype(np.float64), "rms", 1.0, 0.0, np.float64(np.float32(1e-6))), F32))
 
 
+#: (d, sequences, rows of one): more rows than are on the GPU at once, both sides of a warp's, of a team's and of the teams' largest width
+MANY_ROWS = [(7, 2, 1500), (8, 3, 1700), (9, 1, 5000), (100, 4, 1000), (383, 3, 1001), (384, 2, 1500), (512, 5, 500), (513, 1, 2000), (520, 4, 400), (1000, 3, 301),
+             (2560, 7, 100), (2561, 2, 351), (4104, 1, 333), (5001, 3, 67), (8191, 2, 75), (8192, 1, 151), (8193, 1, 77), (9001, 2, 40), (10240, 3, 33), (10248, 1, 50)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("post,pre", [("rms", "rms"), ("layer", "layer"), (None, "layer"), ("rms", None)])
+def test_residual_norm_of_many_rows(dt, post, pre, gpu):
+    f64 = lambda v: None if v is None else v.astype(np.float64)  # noqa: E731
+    for i, (d, sequences, rows) in enumerate(MANY_ROWS):
+        rng = np.random.default_rng(2000 + d)
+        r, y = (round_to(dt, (s * rng.standard_normal((sequences, rows, d), dtype=np.float32))) for s in (3.0, 1.0))
+        gate = round_to(dt, rng.uniform(-1, 1, [(sequences, 1, d), (d,)][i % 2]).astype(np.float32)) if i % 3 else None
+        pp, post_t = norm_weights(post, d, F32 if i % 4 == 3 else dt, rng)
+        qq, pre_t = norm_weights(pre, d, dt, rng)
+        mod = ResidualNorm(norm_module(pre, qq, gpu, dt), norm_module(post, pp, gpu, F32 if i % 4 == 3 else dt), 0.75, -1.25)
+        h, x = mod.schedule(*(None if v is None else Tensor.from_data(v, gpu, dt) for v in (r, y, gate)))
+        th, tx = norm_truth(f64(r), f64(y), f64(gate), post_t, pre_t, 0.75, -1.25)
+        assert np.all(close(h.resolve().to(Device.CPU).to_f32(), th, dt)), (d, "h")
+        if x is not None:
+            assert np.all(close(x.resolve().to(Device.CPU).to_f32(), tx, dt)), (d, "x")
+        if post is None:
+            alone = mod.pre.schedule(Tensor.from_data(r, gpu, dt)).resolve().to(Device.CPU).to_f32()
+            assert np.all(close(alone, normed(f64(r), 0 * f64(r), *pre_t), dt)), (d, "alone")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,ld,shift,rows", [(64, 72, 0, 4001), (64, 67, 1, 4001), (9, 9, 3, 6000), (9, 16, 0, 6000), (384, 1160, 8, 2500), (1001, 1001, 0, 900), (1001, 1003, 5, 900),
+                                             (1000, 1003, 0, 900), (2560, 2560, 0, 400)])
+def test_many_strided_rows_in_place(d, ld, shift, rows, gpu):
+    """h over the block, x over the residual, while later rows are on their way; nothing between, before or behind the rows is touched."""
+    rng = np.random.default_rng(18)
+    for kind in (_lib.RT_NORM_RMS, _lib.RT_NORM_LAYER):
+        mats = [round_to(F16, rng.standard_normal(rows * ld + shift + 11).astype(np.float32)).astype(np.float16) for _ in range(2)]
+        bufs = [device_array(gpu, m) for m in mats]
+        w = device_array(gpu, np.ones(d, np.float16))
+        p = _lib.rt_residual_norm()
+        p.dt, p.residual_scale, p.block_scale, p.rows, p.d = _lib.RT_F16, 0.5, 2.0, rows, d
+        p.residual, p.block = bufs[0].ptr + 2 * shift, bufs[1].ptr + 2 * shift
+        p.h, p.x = p.block, p.residual
+        p.residual_ld = p.block_ld = p.h_ld = p.x_ld = ld
+        p.pre.kind, p.pre.dt, p.pre.eps, p.pre.weight = kind, _lib.RT_F16, 1e-5, w.ptr
+        _lib.check(_lib.load().rt_residual_norm_launch(gpu._h, ctypes.byref(p), None))
+        x, h = [read_back(gpu, b, m) for b, m in zip(bufs, mats)]
+        at = (shift + np.arange(rows)[:, None] * ld + np.arange(d)[None, :]).reshape(-1)
+        r, y = (m[at].reshape(rows, d).astype(np.float64) for m in mats)
+        truths = norm_truth(r, y, None, (None, 1.0, 0.0, 0.0), ("rms" if kind == _lib.RT_NORM_RMS else "layer", np.ones(d), 0.0, np.float64(np.float32(1e-5))), 0.5, 2.0)
+        for g, m, t in zip((h, x), (mats[1], mats[0]), truths):
+            assert np.all(close(g[at].reshape(rows, d).astype(np.float32), t, F16)), kind
+            rest = np.ones(m.size, bool)
+            rest[at] = False
+            assert np.array_equal(g[rest], m[rest])
+
+
+@pytest.mark.gpu
+def test_what_is_not_finite_stays_in_its_row_of_many(gpu):
+    rng = np.random.default_rng(19)
+    for d in (300, 304, 1203):
+        r, y = rng.standard_normal((2, 3000, d)).astype(np.float32)
+        w = Tensor.from_data(np.ones(d, np.float32), gpu)
+        for mod in (ResidualNorm(LayerNorm(w), RMSNorm(w)), ResidualNorm(RMSNorm(w))):
+            run = lambda a, b: [t.resolve().to(Device.CPU).to_f32() for t in mod.schedule(Tensor.from_data(a, gpu), Tensor.from_data(b, gpu))]  # noqa: E731
+            clean = run(r, y)
+            r2, y2 = r.copy(), y.copy()
+            bad = np.array([0, 7, 8, 1501, 2999])
+            r2[bad[:3], d - 1], y2[bad[3:], 2] = np.inf, np.nan
+            rest = np.delete(np.arange(3000), bad)
+            for c, b in zip(clean, run(r2, y2)):
+                assert np.array_equal(c[rest], b[rest]) and not np.isfinite(b[bad]).all(-1).any()
+
+
 # ------------------------------------------------------------------------------------------------ GPU: log probabilities
 
 def lp_truth(v):
