@@ -43,6 +43,7 @@ struct Q4GroupParams {
     int lhs_constant;
     int fours;      // the groups of a row in a CTA's K range come in aligned fours
     uint32_t magic; // ceil(2^32 / n) for the number of these (or of groups) in a row
+    uint32_t nv_magic; // and for nv
     uint32_t xsum_at, up_at, scales_at, part_at; // bytes into shared memory (activations at 0)
 };
 
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
 
     // ---- scales of the rows' groups in this K range, 0 (a group that adds nothing) past K: four groups of a row at a time where
     // their number allows it, the first FOURS of a thread asked for before it waits for the stream predecessor
-    constexpr int FOURS = 3;
+    constexpr int FOURS = 4;
     const int row_groups = K >> p.lhs_group_shift, left = min(n_steps * G, row_groups - first * G);
     const long long scale0 = lhs_row * row_groups + first * G;
     const uint16_t *const s16 = (const uint16_t *)p.lhs_scales + scale0;
@@ -217,10 +218,10 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     };
     uint2 s4[FOURS];
     uint32_t z4[FOURS];
-    if (q.fours) {
+    auto load_fours = [&](int from) {
 #pragma unroll
         for (int k = 0; k < FOURS; k++) {
-            const int e = tid + k * (int)blockDim.x;
+            const int e = from + k * (int)blockDim.x;
             s4[k] = make_uint2(0, 0), z4[k] = 0;
             if (e >= n_units) continue;
             int i;
@@ -232,39 +233,37 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
                 z4[k] = __ldg(reinterpret_cast<const uint32_t *>(z8 + at));
             }
         }
-    }
+    };
+    if (q.fours) load_fours(tid);
     if (q.lhs_constant) asm volatile("griddepcontrol.wait;" ::: "memory");
     const T *const x = (const T *)p.rhs + (long long)(p.rhs_stack == 1 ? 0 : batch) * q.nv * K;
-    const int n_x = n_steps * NVS * 16; // eight values each; vectors past nv are passed over
-    auto load_x = [&](int e) {
-        const int sv = e >> 4, v = sv % NVS, k = (first + sv / NVS) * STEP + (e & 15) * 8;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (e < n_x && v < q.nv && k < K) raw = *reinterpret_cast<const uint4 *>(x + ((uint32_t)v * (uint32_t)K + (uint32_t)k));
-        return raw;
-    };
-    uint4 raw = load_x(tid);
-    if (q.fours) {
+    constexpr int XA = NVS > 8 ? 3 : NVS > 1 ? 2 : 1; // asked for together
+    const int n_x = n_steps * q.nv * 16; // eight values each
+    auto step_of = [&](int sv) { return NVS <= 2 ? sv / NVS : (int)__umulhi((uint32_t)sv, q.nv_magic); }; // (nv = NVS up to 2)
+    uint4 raw[XA];
+    auto load_x = [&](int from) {
 #pragma unroll
-        for (int k = 0; k < FOURS; k++) {
-            const int e = tid + k * (int)blockDim.x;
-            if (e >= n_units) continue;
-            int i;
-            bool there;
-            const int place = place_of(e, i, there);
-            put_four(place, i, s4[k], z4[k]);
+        for (int i = 0; i < XA; i++) {
+            const int e = from + i * (int)blockDim.x, sv = e >> 4, step = step_of(sv), v = sv - step * q.nv, k = (first + step) * STEP + (e & 15) * 8;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (e < n_x && k < K) raw[i] = *reinterpret_cast<const uint4 *>(x + ((uint32_t)v * (uint32_t)K + (uint32_t)k));
         }
-        for (int e = tid + FOURS * (int)blockDim.x; e < n_units; e += blockDim.x) {
-            int i;
-            bool there;
-            const int place = place_of(e, i, there);
-            uint2 s = make_uint2(0, 0);
-            uint32_t z = 0;
-            if (there && 4 * i < left) {
-                const long long at = source(place) + 4 * i;
-                s = __ldg(reinterpret_cast<const uint2 *>(s16 + at));
-                z = __ldg(reinterpret_cast<const uint32_t *>(z8 + at));
+    };
+    load_x(tid);
+    if (q.fours) {
+        for (int from = tid;;) {
+#pragma unroll
+            for (int k = 0; k < FOURS; k++) {
+                const int e = from + k * (int)blockDim.x;
+                if (e >= n_units) continue;
+                int i;
+                bool there;
+                const int place = place_of(e, i, there);
+                put_four(place, i, s4[k], z4[k]);
             }
-            put_four(place, i, s, z);
+            from += FOURS * (int)blockDim.x;
+            if (from >= n_units) break;
+            load_fours(from);
         }
     } else {
 #pragma unroll 4
@@ -284,10 +283,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     // ---- activations: 16 threads take a step of one vector, 8 values each.  bf16 values come into f16's range with a power of two
     // per step and vector, which the sums are multiplied by again: nothing saturates, and a value that loses bits is 2^-24 of
     // its step's largest or less.
-    for (int e = tid; e < (n_x + 31) / 32 * 32; e += blockDim.x) { // (whole warps, for the shuffles)
-        const int u = e & 15, sv = e >> 4, step = sv / NVS, v = sv % NVS;
-        if (e != tid) raw = load_x(e);
-        uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    auto put_x = [&](int e, const uint4 &of) {
+        const int u = e & 15, sv = e >> 4, step = step_of(sv), v = sv - step * q.nv;
+        uint32_t w[4] = {of.x, of.y, of.z, of.w};
         if (BF16) {
             uint32_t top = 0; // the largest finite magnitude's bits
 #pragma unroll
@@ -302,7 +300,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
             const float down = __uint_as_float((uint32_t)(127 - sh) << 23);
 #pragma unroll
             for (int i = 0; i < 4; i++) w[i] = bf16x2_to_f16x2(w[i], down);
-            if (u == 0 && e < n_x) up[sv] = __uint_as_float((uint32_t)(127 + sh) << 23);
+            if (u == 0 && e < n_x) up[step * NVS + v] = __uint_as_float((uint32_t)(127 + sh) << 23);
         }
         float sum = 0.f;
 #pragma unroll
@@ -320,6 +318,14 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
                                                                  __byte_perm(w[0], w[2], 0x7632), __byte_perm(w[1], w[3], 0x7632));
             if (u % (16 / G) == 0) xsum[(step * G + u / (16 / G)) * NVS + v] = sum;
         }
+    };
+    for (int from = tid;;) {
+#pragma unroll
+        for (int i = 0; i < XA; i++)
+            if (from + i * (int)blockDim.x < (n_x + 31) / 32 * 32) put_x(from + i * (int)blockDim.x, raw[i]); // (whole warps, for the shuffles)
+        from += XA * (int)blockDim.x;
+        if (from >= (n_x + 31) / 32 * 32) break;
+        load_x(from);
     }
     __syncthreads();
 
@@ -594,6 +600,7 @@ cudaError_t launch_q4_group_gemv(const MatmulParams &p, rt_dtype act, int nv, in
     q.fours = p.K / group % 4 == 0 && per_row % 4 == 0;
     const int n = q.fours ? per_row / 4 : per_row;
     q.magic = n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0u;
+    q.nv_magic = nv > 1 ? (uint32_t)(((1ull << 32) + nv - 1) / nv) : 0u;
     return act == RT_F16 ? launch_t<__half>(q, c, batches, stream) : launch_t<__nv_bfloat16>(q, c, batches, stream);
 }
 
