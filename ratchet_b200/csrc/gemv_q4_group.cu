@@ -16,6 +16,10 @@
 //  * Activations are staged in shared memory in the order the MMAs take them, with their sums by group; so are scales and zero
 //    points, a word a group (read from global memory by the lanes that need them they would be more requests than the codes).
 //  * f32 sums of a group times s, added in f32 over steps, warps and CTAs of the cluster in a fixed order.
+//
+// One vector, 51200 rows of 2560: 15.7 us with groups of 128 (4.4 TB/s), 17.2 of 64, 19.1 of 32; 2560 x 2560 3.8, the launch and two
+// trips to memory; 16 vectors 25.4 / 31 / 48: the epilogue of a group (FMAs by vectors) and the masking bound those.  A CUDA-core
+// product of the same layout took 5 to 80 times as long (2560 x 10240 with 5 vectors: 841 us against 10.0).
 #include <algorithm>
 
 #include "common.cuh"
@@ -193,7 +197,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     for (int a = 0; a < AHEAD; a++) load(code[a], code0 + a * (STEP / 2), begin + a < end);
 
     // ---- scales of the rows' groups in this K range, 0 (a group that adds nothing) past K: four groups of a row at a time where
-    // their number allows it, the first FOURS of a thread asked for before it waits for the stream predecessor
+    // their number allows it, FOURS of a thread asked for together, the first ones before it waits for the stream predecessor
+    // (51200 x 2560, groups of 32, one vector: 19.1 us, 20.5 where the later ones came one by one)
     constexpr int FOURS = 4;
     const int row_groups = K >> p.lhs_group_shift, left = min(n_steps * G, row_groups - first * G);
     const long long scale0 = lhs_row * row_groups + first * G;
@@ -280,8 +285,8 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
         }
     }
 
-    // ---- activations: 16 threads take a step of one vector, 8 values each.  bf16 values come into f16's range with a power of two
-    // per step and vector, which the sums are multiplied by again: nothing saturates, and a value that loses bits is 2^-24 of
+    // ---- activations: 16 threads take a step of one vector, 8 values each, XA of them asked for together (4096 x 8192, bf16, 5
+    // vectors: 10.8 us, 11.5 one by one).  bf16 values come into f16's range with a power of two per step and vector, which the sums are multiplied by again: nothing saturates, and a value that loses bits is 2^-24 of
     // its step's largest or less.
     auto put_x = [&](int e, const uint4 &of) {
         const int u = e & 15, sv = e >> 4, step = step_of(sv), v = sv - step * q.nv;
@@ -517,7 +522,7 @@ template <typename T> cudaError_t launch_t(const Q4GroupParams &q, const Q4Group
     }
 }
 
-constexpr size_t MOST_SMEM = 220u << 10, HALF_SMEM = 80u << 10; // for a CTA that has an SM to itself, or half of one
+constexpr size_t MOST_SMEM = 220u << 10, HALF_SMEM = 32u << 10; // for a CTA that has an SM to itself, or half of one
 
 // The sizes that follow from units, parts and ranks; false when they do not fit.
 bool complete(Q4GroupConfig &c, int M, int K, int group, int nv, bool pair) {
@@ -546,8 +551,11 @@ bool complete(Q4GroupConfig &c, int M, int K, int group, int nv, bool pair) {
 } // namespace
 
 // How rows and K are shared out.  Counted in steps of a tile (16 rows x 128 values) that an SM has to work off one after the
-// other: with few rows the tiles do not divide evenly among the SMs, and a K range of the tiles shared by a cluster's CTAs does,
-// for the price of two cluster barriers; activations that every CTA stages count as well.
+// other: with few rows the tiles do not divide evenly among the SMs, and a K range of the tiles shared by a cluster's CTAs does;
+// activations that every CTA stages count as well, more where they take many rounds, and a cluster's start and two barriers as 55
+// or 80 steps; the weights are fitted to what these products took.  2560 x 10240 with 8 vectors: 21.0 us without clusters, 12.3 in
+// twos, 10.6 in fours; 2560 x 2560: 5.2, 5.2, 6.6; 20000 x 4096 with 16: 36, 27, and fours not better.
+// Clusters of eight are left out: with a CTA an SM few of them are resident (2560 x 2560, one vector: 18.7 us, 3.7 without).
 bool q4_group_gemv_config(int M, int K, int group, int nv, int batches, bool pair, int sm_count, Q4GroupConfig *out) {
     const int steps = (K + STEP - 1) / STEP, nvs = nv <= 2 ? nv : nv <= 4 ? 4 : nv <= 8 ? 8 : 16;
     const long long tiles = (long long)(pair ? (M / 2 + 7) / 8 : (M + 15) / 16) * batches;
@@ -564,9 +572,12 @@ bool q4_group_gemv_config(int M, int K, int group, int nv, int batches, bool pai
         c.parts = std::min(per, std::max(1, 20 / c.units));
         while (!complete(c, M, K, group, nv, pair) && c.units > 1) c.units = (c.units + 1) / 2, c.parts = std::min(per, std::max(1, 20 / c.units));
         if (!complete(c, M, K, group, nv, pair)) continue;
-        const double cost = (double)per_sm * per * (nvs > 8 ? 2 : 1) + (double)per * nvs * 16 / 640 * 6 + (ranks > 1 ? 30 : 0);
+        const double staged = (double)per * nv * 16 / 640; // 16-byte pieces of activations a thread
+        const double cost = (double)per_sm * per * (nvs > 8 ? 2 : 1) + 6 * staged + 8 * std::max(0.0, staged - (nvs > 8 ? 8 : 4)) +
+                            (ranks == 4 ? 80 : ranks == 2 ? 55 : 0);
         if (found && cost >= best) continue;
-        // two CTAs to an SM where they fit: one stages while the other works
+        // two CTAs to an SM, of which one stages while the other works, where they stage little (51200 x 2560, groups of 128: one
+        // vector 15.7 us, 16.4 as one CTA; 8 vectors, 55 KB each, 19.6 and 18.9; 16, 102 KB each, 31 and 25)
         if (c.units >= MAX_WARPS / 2 && ranks == 1) {
             Q4GroupConfig two = c;
             two.units = (c.units + 1) / 2;
