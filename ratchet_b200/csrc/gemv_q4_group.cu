@@ -554,7 +554,7 @@ bool complete(Q4GroupConfig &c, int M, int K, int group, int nv, bool pair) {
 // other: with few rows the tiles do not divide evenly among the SMs, and a K range of the tiles shared by a cluster's CTAs does;
 // activations that every CTA stages count as well, more where they take many rounds, and a cluster's start and two barriers as 55
 // or 80 steps; the weights are fitted to what these products took.  2560 x 10240 with 8 vectors: 21.0 us without clusters, 12.3 in
-// twos, 10.6 in fours; 2560 x 2560: 5.2, 5.2, 6.6; 20000 x 4096 with 16: 36, 27, and fours not better.
+// twos, 10.6 in fours; 2560 x 2560: 5.2, 5.2, 6.6; 20000 x 4096 with 16: 36 and 27 in twos.
 // Clusters of eight are left out: with a CTA an SM few of them are resident (2560 x 2560, one vector: 18.7 us, 3.7 without).
 bool q4_group_gemv_config(int M, int K, int group, int nv, int batches, bool pair, int sm_count, Q4GroupConfig *out) {
     const int steps = (K + STEP - 1) / STEP, nvs = nv <= 2 ? nv : nv <= 4 ? 4 : nv <= 8 ? 8 : 16;

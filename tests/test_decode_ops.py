@@ -671,3 +671,81 @@ def test_calls_on_other_streams_and_in_a_captured_graph(gpu):
         torch.cuda.synchronize()
         right(cases[0])
     del graph
+
+
+@pytest.mark.gpu
+def test_many_rows_on_two_streams_and_in_a_replayed_graph(gpu):
+    """Teams that walk rows, two launches at once on one device, and a captured one on changed inputs."""
+    import torch
+    lib, cases = _lib.load(), []
+    for d, rows in ((520, 3000), (1001, 1200)):
+        r, y = torch.randn(2, rows, d, generator=torch.Generator().manual_seed(d)).cuda()
+        w, h, x = torch.ones(d, device="cuda"), torch.zeros_like(r), torch.zeros_like(r)
+        n = _lib.rt_residual_norm()
+        n.dt, n.residual_scale, n.block_scale, n.rows, n.d, n.gate_rows = _lib.RT_F32, 1, 1, rows, d, 1
+        n.residual, n.block, n.h, n.x = r.data_ptr(), y.data_ptr(), h.data_ptr(), x.data_ptr()
+        n.residual_ld = n.block_ld = n.h_ld = n.x_ld = d
+        n.pre.kind, n.pre.dt, n.pre.eps, n.pre.weight = _lib.RT_NORM_RMS, _lib.RT_F32, 1e-5, w.data_ptr()
+        cases.append((r, y, h, x, n, w))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    launch = lambda case, stream: _lib.check(lib.rt_residual_norm_launch(gpu._h, ctypes.byref(case[4]), stream.cuda_stream))  # noqa: E731
+
+    def right(case):
+        r, y, h, x = case[:4]
+        hv = (r.double() + y.double()).cpu().numpy()
+        assert np.all(close(h.cpu().numpy(), (hv, 0 * hv), F32))
+        assert np.all(close(x.cpu().numpy(), normed(hv, E24 * np.abs(hv), "rms", 1.0, 0.0, np.float64(np.float32(1e-5))), F32))
+
+    for _ in range(20):
+        for case, stream in zip(cases, streams):
+            launch(case, stream)
+    torch.cuda.synchronize()
+    for case in cases:
+        right(case)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for case in cases:
+            launch(case, torch.cuda.current_stream())
+    for _ in range(3):
+        for case in cases:
+            case[0].normal_()
+            case[1].mul_(1.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        for case in cases:
+            right(case)
+    del graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("d", [96, 520, 1003])
+def test_many_gates(d, dt, gpu):
+    """A gate per row, per seven rows and per sequence of many rows: a team's rows cross from one to the next."""
+    rng = np.random.default_rng(51)
+    r, y = (round_to(dt, rng.standard_normal((70, 7, 9, d), dtype=np.float32)) for _ in range(2))
+    pre, pre_t = norm_weights("layer", d, dt, rng)
+    post, post_t = norm_weights("rms", d, dt, rng)
+    mod = ResidualNorm(norm_module("layer", pre, gpu, dt), norm_module("rms", post, gpu, dt))
+    for shape in ((70, 7, 9, d), (70, 7, 1, d), (70, 1, 1, d), (1, 1, 1, d)):
+        gate = round_to(dt, rng.standard_normal(shape, dtype=np.float32))
+        h, x = mod.schedule(*(Tensor.from_data(v, gpu, dt) for v in (r, y, gate)))
+        th, tx = norm_truth(*(v.astype(np.float64) for v in (r, y, gate)), post_t, pre_t, 1.0, 1.0)
+        assert np.all(close(h.resolve().to(Device.CPU).to_f32(), th, dt)) and np.all(close(x.resolve().to(Device.CPU).to_f32(), tx, dt)), shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,vocab", [(F32, 262143), (F32, 300001), (F32, 524289), (F16, 262145), (F16, 600011), (BF16, 1100003)])
+def test_vocabularies_that_a_cluster_s_ctas_share(dt, vocab, gpu):
+    """One to three rows of more tokens than a CTA takes alone: the likeliest at the ends of the CTAs' shares, and with nothing else."""
+    for rows, top in ((1, 32), (3, 5), (2, 0)):
+        rng = np.random.default_rng(vocab + rows)
+        v = round_to(dt, (2.5 * rng.standard_normal((rows, vocab))).astype(np.float32))
+        at = [vocab * k // 8 + e for k in range(9) for e in (-1, 0, 1) if 0 <= vocab * k // 8 + e < vocab]
+        v[0, at] = round_to(dt, (14 + 4 * rng.random(len(at))).astype(np.float32))
+        if rows > 1:
+            v[1] = -np.inf
+            v[1, [0, vocab - 1]] = 1.0
+        tokens = [0] * rows if rows != 2 else None
+        lp_check(v, tokens, top, gpu, dt)

@@ -311,3 +311,142 @@ def test_empty_products(gpu):
     w, _ = weight(G32, (8, 64), 19)
     y = Linear(w.to(gpu)).schedule(Tensor.from_data(np.zeros((1, 0, 64), np.float16), gpu)).resolve()
     assert y.shape == [1, 0, 8]
+
+
+# What a product's kernel is called depends on the GPU's number of SMs in the last part only (how rows and K are shared out).
+
+def product(w, wv, x, act, gpu, bias=None, epilogue=rb.EPILOGUE_NONE):
+    """(result, 64-bit sums, how far off they may be, kernel)"""
+    y = x[0].astype(np.float64) @ wv.T + (0 if bias is None else bias)
+    got, kernel = run(w, x, act, gpu, bias, epilogue)
+    return got[0], y, error_bound(act, wv, x[0].astype(np.float64), y, bias, "umma" in kernel), kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [F16, BF16])
+@pytest.mark.parametrize("m,k,rows,ranks", [(16, 5120, 8, 2), (50, 5120, 7, 2), (16, 3200, 16, 4), (130, 3232, 13, 1), (200, 6432, 15, 4), (25, 10272, 16, 4), (16, 25600, 1, None), (40, 20480, 3, None)])
+def test_k_shared_by_warps_and_by_a_cluster(m, k, rows, ranks, act, gpu):
+    """Few rows of great length, the last step partial or a whole CTA's share shorter; infinities there as well."""
+    w, wv = weight(G32, (m, k), 31)
+    x = activations(act, (1, rows, k), 32)
+    got, y, e, kernel = product(w, wv, x, act, gpu)
+    assert kernel.startswith(f"q4_group_gemv_g32_nv{rows}_") and (ranks is None or f"x{ranks}_" in kernel), kernel
+    assert np.all(np.abs(got - y) <= e), kernel
+    x[0, rows - 1, k - 1] = np.inf
+    bad, _ = run(w, x, act, gpu)
+    with np.errstate(invalid="ignore"):
+        assert np.array_equal(bad[0, :-1], got[:-1]) and np.array_equal(bad[0, -1], (np.inf * wv[:, k - 1]).astype(np.float32), equal_nan=True), kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 4, 8, 12, 16])
+def test_k_that_is_no_multiple_of_a_step(rows, gpu):
+    for dt, k in ((G32, 32), (G32, 96), (G32, 160), (G32, 2592), (G64, 64), (G64, 192), (G64, 2624)):
+        w, wv = weight(dt, (37, k), k)
+        for act in (F16, BF16):
+            got, y, e, kernel = product(w, wv, activations(act, (1, rows, k), 33), act, gpu)
+            assert np.all(np.abs(got - y) <= e), (kernel, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,m", [(12, 16), (16, 16), (9, 300), (12, 2)])
+def test_rows_too_long_for_the_gemv(rows, m, gpu):
+    """25600 values of 9 and more vectors do not fit its shared memory: the general routes take them, with the fold as well."""
+    w, wv = weight(G128, (m, 25600), 34)
+    x = activations(F16, (1, rows, 25600), 35)
+    got, y, e, kernel = product(w, wv, x, F16, gpu)
+    assert "q4_group_gemv" not in kernel and np.all(np.abs(got - y) <= e), kernel
+    fold, kernel = run(w, x, F16, gpu, None, rb.EPILOGUE_SILU_MUL)
+    gate, up, eg, eu = y[:, :m // 2], y[:, m // 2:], e[:, :m // 2], e[:, m // 2:]
+    silu = gate / (1 + np.exp(-gate))
+    es = 1.1 * eg + (2.0**-11 + 2.0**-20) * np.abs(silu) + 2.0**-24
+    bound = es * (np.abs(up) + eu) + np.abs(silu) * eu + 2.0**-11 * (np.abs(silu * up) + es * np.abs(up)) * 1.02 + 2.0**-24
+    assert np.all(np.abs(fold[0] - silu * up) <= bound), kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 5, 20])
+def test_the_cuda_core_kernel_s_bits_are_within_the_same_bounds(rows, act, gpu, monkeypatch):
+    monkeypatch.setenv("RT_FORCE_KERNEL", "simt")
+    for dt in GROUP:
+        w, wv = weight(dt, (70, 3 * GROUP[dt]), 36)
+        x = activations(act, (1, rows, 3 * GROUP[dt]), 37)
+        bias = round_to(act, np.random.default_rng(38).standard_normal(70).astype(np.float32)).astype(np.float64)
+        got, y, e, kernel = product(w, wv, x, act, gpu, bias)
+        assert "simt" in kernel and np.all(np.abs(got - y) <= e), kernel
+        fold, kernel = run(w, x, act, gpu, bias, rb.EPILOGUE_SILU_MUL)
+        gate, up = y[:, :35], y[:, 35:]
+        silu, u = gate / (1 + np.exp(-gate)), HALF_STEP[act]
+        es = 1.1 * e[:, :35] + (u + 2.0**-20) * np.abs(silu) + 2.0**-24
+        bound = es * (np.abs(up) + e[:, 35:]) + np.abs(silu) * e[:, 35:] + u * (np.abs(silu * up) + es * np.abs(up)) * 1.02 + 2.0**-24
+        assert "simt" in kernel and np.all(np.abs(fold[0] - silu * up) <= bound), kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 8, 16])
+@pytest.mark.parametrize("scale", [1e-36, 1e-30, 1e-8, 1e8, 1e30, 1e36])
+def test_bf16_activations_of_every_size(scale, rows, gpu):
+    """Every step of a vector has a power of two of its own: sizes that f16 does not have, and steps that differ by 2^40."""
+    for dt in GROUP:
+        k = 640
+        w, wv = weight(dt, (48, k), 39)
+        x = np.random.default_rng(40).standard_normal((1, rows, k)) * scale
+        if scale < 1:
+            x[..., 128:256] *= 2.0**-20
+            x[..., 256:384] *= 2.0**20
+        x = round_to(BF16, x.astype(np.float32))
+        v = x[0].astype(np.float64)
+        y = v @ wv.T
+        got, kernel = run(w, x, BF16, gpu)
+        # a value that leaves f16's range below loses 2^-24 of its step's largest or less: 2^-25 of a step's largest magnitude for each of its weights
+        steps = np.abs(v).reshape(rows, -1, 128).max(-1)
+        lost = np.einsum("ns,ms->nm", steps, np.abs(wv).reshape(48, -1, 128).sum(-1)) * 2.0**-24
+        e = HALF_STEP[BF16] * np.abs(y) * (1 + 2.0**-6) + (np.abs(v) @ np.abs(wv).T) * ((k + 8) * 2.0**-24) + lost + 2.0**-133
+        assert np.all(np.abs(got[0] - y) <= e), (kernel, float((np.abs(got[0] - y) - e).max()))
+
+
+@pytest.mark.gpu
+def test_the_gemv_on_two_streams_and_in_a_replayed_graph(gpu):
+    import torch
+    lib = _lib.load()
+    w, wv = weight(G32, (130, 3232), 41)
+    w2, wv2 = weight(G64, (200, 640), 42)
+    cases = []
+    for wt, vals, rows in ((w, wv, 13), (w2, wv2, 1)):
+        k = vals.shape[1]
+        x = torch.randn(rows, k, generator=torch.Generator().manual_seed(rows)).half().cuda()
+        dev = Linear(wt.to(gpu))
+        plan = gpu.plan_for(dev.schedule(Tensor.from_data(np.zeros((1, rows, k), np.float32), gpu, F16)).op.desc)
+        cases.append((dev, plan, x, torch.zeros(rows, vals.shape[0], dtype=torch.half, device="cuda"), vals))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+
+    def launch(case, stream):
+        dev, plan, x, out, _ = case
+        _lib.check(lib.rt_matmul_launch(plan, dev.w.ptr, x.data_ptr(), None, out.data_ptr(), stream.cuda_stream))
+
+    def right(case):
+        _, _, x, out, vals = case
+        v = x.double().cpu().numpy()
+        y = v @ vals.T
+        assert np.all(np.abs(out.double().cpu().numpy() - y) <= error_bound(F16, vals, v, y))
+
+    for _ in range(20):
+        for case, stream in zip(cases, streams):
+            launch(case, stream)
+    torch.cuda.synchronize()
+    for case in cases:
+        right(case)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for case in cases:
+            launch(case, torch.cuda.current_stream())
+    for _ in range(3):
+        for case in cases:
+            case[2].normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for case in cases:
+            right(case)
+    del graph
