@@ -10,8 +10,10 @@
 //
 // 8192 bf16 rows of 2560, rms on both sides, a gate a sequence: 33.0 us, 5.1 TB/s (a CTA a row without the ring: 44; with means and
 // biases 44.8: four sums a row instead of two, 128 registers instead of 96).  What is left is instructions, 1.9 a cycle and SM with
-// 20 warps, and the start.  Rows of 2561, value by value: 71 us.  One row: 3.4 us, the launch.
+// 20 warps, and the start.  Rows of 2561, all off the 16-byte boundary, with a sixth warp for one value: 53 us.  One row: 3.4 us, the
+// launch.
 #include <algorithm>
+#include <utility>
 
 #include "common.cuh"
 #include "f32x2.cuh"
@@ -59,6 +61,16 @@ template <typename T, int VEC> struct Values {
 #pragma unroll
         for (int i = 0; i < WORDS; i++) raw[i] = lds128(a + 16 * i);
     }
+    __device__ __forceinline__ void keep(int from, int to) { // 0 but for values from .. to - 1
+        constexpr int PER = 4 / sizeof(T);
+        uint32_t *const w = reinterpret_cast<uint32_t *>(raw);
+#pragma unroll
+        for (int k = 0; k < 4 * WORDS; k++) {
+            const uint32_t low = k * PER >= from && k * PER < to ? PER == 2 ? 0xffffu : 0xffffffffu : 0u;
+            const uint32_t high = PER == 2 && k * PER + 1 >= from && k * PER + 1 < to ? 0xffff0000u : 0u;
+            w[k] &= low | high;
+        }
+    }
     __device__ __forceinline__ void get(float (&v)[VEC]) const {
 #pragma unroll
         for (int i = 0; i < WORDS; i++) {
@@ -81,6 +93,7 @@ template <typename T> struct Values<T, 1> {
     T raw;
     __device__ __forceinline__ void clear() { raw = from_f32<T>(0.f); }
     __device__ __forceinline__ void load(const T *p) { raw = *p; }
+    __device__ __forceinline__ void keep(int, int) {}
     __device__ __forceinline__ void load_shared(uint32_t a) {
         if constexpr (sizeof(T) == 4) {
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(raw) : "r"(a) : "memory");
@@ -303,30 +316,34 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 // Teams that walk rows, a warp each (blockDim.y of them in a CTA) or the CTA.  A team's rows are consecutive, `share` of them; each warp
 // holds 32 N consecutive values of a row, of which a thread's are VEC every 32 VEC: all but the last warp go without predicates and
 // with constant offsets.  `stages` rows are in shared memory or on their way there.
-// With VEC = 1 rows may start anywhere: the 16-byte words that hold the row are copied, which in the first and the last row
-// would reach outside the tensor: those are read where they are.
+// SHIFT: rows start s values behind a 16-byte boundary, every operand's alike.  s is the same in every `period`-th row, so a team
+// takes such rows only, and its threads' values sit at the same places in each: s values before those of an aligned row.  The
+// 16-byte words that hold the row are copied, which in the first and the last row would reach outside the tensor: those are read where
+// they are.  VEC = 1: the same copies for operands that differ in s, value by value.
 // PLAIN: no means and no biases, which leaves the registers for more teams.
 constexpr int N = 16, MAX_STAGES = 4, MAX_TEAMS = 8, WALK_SMEM = 200 * 1024;
 constexpr int MIN_WALK_D = 8; // 16 bytes: the words of a row that is neither first nor last lie in the tensor
 template <bool PLAIN> constexpr int WALK_THREADS = PLAIN ? 640 : 512; // of an SM, at 96 or 128 registers
 
-template <int VEC> __host__ __device__ constexpr int walk_operand_bytes(int row_bytes) { // of a stage
-    return VEC > 1 ? row_bytes : (row_bytes + 15) / 16 * 16 + 16;
+template <bool ALIGNED> __host__ __device__ constexpr int walk_operand_bytes(int row_bytes) { // of a stage
+    return ALIGNED ? row_bytes : (row_bytes + 15) / 16 * 16 + 16;
 }
 
-template <typename T, int VEC, bool WARP, bool PLAIN>
-__global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, WARP ? 2 : 1) residual_norm_walk_kernel(const __grid_constant__ ResidualNormParams p, int share, int stages) {
+template <typename T, int VEC, bool WARP, bool PLAIN, bool SHIFT>
+__global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, WARP ? 2 : 1) residual_norm_walk_kernel(const __grid_constant__ ResidualNormParams p, int share, int stages, int period) {
     constexpr int C = N / VEC;
+    constexpr bool ALIGNED = VEC > 1 && !SHIFT;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) float red[2][4][32]; // two rows' reductions: a warp may be one row ahead of another
     __shared__ __align__(8) unsigned long long bars[MAX_TEAMS][MAX_STAGES];
     __shared__ int abort_flag;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int t = threadIdx.x, y0 = WARP ? threadIdx.y : 0;
-    const int d = p.d, row_bytes = d * (int)sizeof(T), op_bytes = walk_operand_bytes<VEC>(row_bytes);
+    const int d = p.d, row_bytes = d * (int)sizeof(T), op_bytes = walk_operand_bytes<ALIGNED>(row_bytes);
     const int stage_bytes = op_bytes * ((p.r != nullptr) + (p.y != nullptr));
-    const long long first = ((long long)blockIdx.x * (WARP ? blockDim.y : 1) + y0) * share;
-    const int n = (int)max(0LL, min((long long)share, p.rows - first));
+    const int team = blockIdx.x * (WARP ? blockDim.y : 1) + y0, P = SHIFT ? period : 1; // the team's rows: first, first + P, ..
+    const long long before = (long long)(team / P) * share, first = team % P + before * P;
+    const int n = (int)max(0LL, min((long long)share, (p.rows - team % P + P - 1) / P - before));
     uint32_t bar0 = umma_gemv::smem_u32(&bars[y0][0]), ring0 = umma_gemv::smem_u32(smem) + y0 * stages * stage_bytes, red0 = umma_gemv::smem_u32(red);
     asm volatile("" : "+r"(bar0), "+r"(ring0), "+r"(red0)); // held, not worked out anew in each row
     if (!WARP) clear_sums(red[0], 8);
@@ -338,7 +355,9 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const T *const yp = (const T *)p.y + first * p.y_ld, *const rp = (const T *)p.r + first * p.r_ld;
-    auto in_place = [&](int i) { return VEC == 1 && (first + i == 0 || first + i == p.rows - 1); };
+    const long long y_step = p.y_ld * P, r_step = p.r_ld * P;
+    auto row_of = [&](int i) { return first + (long long)i * P; };
+    auto in_place = [&](int i) { return !ALIGNED && (row_of(i) == 0 || row_of(i) == p.rows - 1); };
     int asked = 0; // rows asked for, by thread 0 of the team
     auto ask = [&](int k) { // the next row, into stage k
         const uint32_t to = ring0 + k * stage_bytes, bar = bar0 + 8 * k;
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
         if (in_place(asked)) {
             mbar_expect(bar, 0);
         } else {
-            const T *const y = yp + asked * p.y_ld, *const r = rp + asked * p.r_ld;
+            const T *const y = yp + asked * y_step, *const r = rp + asked * r_step;
             auto bytes = [&](const T *src) { return (((uint32_t)reinterpret_cast<uintptr_t>(src) & 15) + row_bytes + 15) & ~15u; };
             mbar_expect(bar, (p.y ? bytes(y) : 0) + (p.r ? bytes(r) : 0));
             if (p.y) copy(to, y);
@@ -364,22 +383,27 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
     float mul[N], add[N], wx[N], bx[N];
     float v[VEC];
     const int at0 = (t >> 5) * 32 * N + (t & 31) * VEC;
-    const bool full = (t >> 5) * 32 * N + 32 * N <= d; // the warp's part of the row
+    const int s = SHIFT ? (int)((uint32_t)reinterpret_cast<uintptr_t>(p.y ? yp : rp) & 15) / (int)sizeof(T) : 0;
+    const bool full = (t >> 5) * 32 * N >= s && (t >> 5) * 32 * N + 32 * N <= s + d; // the warp's part of the row
     auto at = [&](int c) { return at0 + c * 32 * VEC; };
+    auto index = [&](int j) { return at(j / VEC) + j % VEC - s; }; // of value j in the row
+    auto valid = [&](int j) { return SHIFT ? (unsigned)index(j) < (unsigned)d : at(j / VEC) < d; };
     auto take_param = [&](const void *from, bool f32, float(&to)[N]) { // all on their way before the first is used; past the row's end its last ones
         auto values = [&](auto *q, auto value) {
-            decltype(value) raw[C];
+            constexpr int W = SHIFT ? 1 : VEC;
+            decltype(value) raw[N / W];
 #pragma unroll
-            for (int c = 0; c < C; c++) raw[c].load(q + min(at(c), d - VEC));
+            for (int c = 0; c < N / W; c++) raw[c].load(q + (SHIFT ? max(0, min(index(c), d - 1)) : min(at(c), d - VEC)));
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                raw[c].get(v);
+            for (int c = 0; c < N / W; c++) {
+                float of[W];
+                raw[c].get(of);
 #pragma unroll
-                for (int j = 0; j < VEC; j++) to[c * VEC + j] = v[j];
+                for (int j = 0; j < W; j++) to[c * W + j] = of[j];
             }
         };
-        if (f32) values((const float *)from, Values<float, VEC>());
-        else values((const T *)from, Values<T, VEC>());
+        if (f32) values((const float *)from, Values<float, SHIFT ? 1 : VEC>());
+        else values((const T *)from, Values<T, SHIFT ? 1 : VEC>());
     };
     auto fill = [&](float(&to)[N], float value) {
 #pragma unroll
@@ -399,20 +423,19 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
         else fill(mul, 1.f);
 #pragma unroll
         for (int j = 0; j < N; j++) { // (past the row's end h stays 0)
-            const float m = at(j / VEC) < d ? p.b * mul[j] : 0.f;
-            mul[j] = at(j / VEC) < d ? m * w[j] : 0.f;
-            add[j] = at(j / VEC) < d ? m * add[j] : 0.f;
+            const float m = valid(j) ? p.b * mul[j] : 0.f;
+            mul[j] = valid(j) ? m * w[j] : 0.f;
+            add[j] = valid(j) ? m * add[j] : 0.f;
         }
     };
-    int gate_rows = 0; // rows left to the gate in the registers
+    long long gate_end = 0; // first row of the gate behind the one in the registers
     T *hp = (T *)p.h + first * p.h_ld, *xp = (T *)p.x + first * p.x_ld;
-    for (int i = 0, k = 0, phase = 0; i < n; i++, hp += p.h_ld, xp += p.x_ld) {
-        if (gate_rows == 0) {
-            const int row = (int)first + i;
-            gate_rows = p.rows_per_gate ? p.rows_per_gate - row % p.rows_per_gate : n;
-            take_gate(p.rows_per_gate ? row / p.rows_per_gate : 0);
+    for (int i = 0, k = 0, phase = 0; i < n; i++, hp += p.h_ld * P, xp += p.x_ld * P) {
+        if (row_of(i) >= gate_end) {
+            const int which = p.rows_per_gate ? (int)row_of(i) / p.rows_per_gate : 0;
+            gate_end = p.rows_per_gate ? (which + 1LL) * p.rows_per_gate : p.rows;
+            take_gate(which);
         }
-        gate_rows--;
         Values<T, VEC> r[C], y[C];
         auto each = [&](auto &&live, auto &&dead) {
             if (full) {
@@ -421,21 +444,31 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
             } else {
 #pragma unroll
                 for (int c = 0; c < C; c++)
-                    if (at(c) < d) live(c);
+                    if (at(c) < s + d) live(c);
                     else dead(c);
             }
         };
+        auto whole = [&](int c) { return !SHIFT || (index(c * VEC) >= 0 && index(c * VEC) + VEC <= d); }; // an access without a neighbour's values
+        auto own = [&](Values<T, VEC> &of, int c) {
+            if (!full && !whole(c)) of.keep(-index(c * VEC), d - index(c * VEC));
+        };
+        auto one_by_one = [&](const T *from, Values<T, VEC> &to, int c) { // an access's values that are the row's
+            alignas(16) T of[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; j++) of[j] = valid(c * VEC + j) ? from[index(c * VEC + j)] : from_f32<T>(0.f);
+            memcpy(&to.raw, of, sizeof(to.raw));
+        };
         umma_gemv::mbar_wait_flag(bar0 + 8 * k, phase, &abort_flag, 1);
-        const T *const ry = yp + i * p.y_ld, *const rr = rp + i * p.r_ld;
+        const T *const ry = yp + i * y_step, *const rr = rp + i * r_step;
         if (in_place(i)) {
-            if (p.y) each([&](int c) { y[c].load(ry + at(c)); }, [&](int c) { y[c].clear(); });
-            if (p.r) each([&](int c) { r[c].load(rr + at(c)); }, [&](int c) { r[c].clear(); });
+            if (p.y) each([&](int c) { one_by_one(ry, y[c], c); }, [&](int c) { y[c].clear(); });
+            if (p.r) each([&](int c) { one_by_one(rr, r[c], c); }, [&](int c) { r[c].clear(); });
         } else {
             const uint32_t from = ring0 + k * stage_bytes + at0 * (int)sizeof(T);
             const uint32_t ys = from + (VEC > 1 ? 0 : (uint32_t)reinterpret_cast<uintptr_t>(ry) & 15);
             const uint32_t rs = from + (p.y ? op_bytes : 0) + (VEC > 1 ? 0 : (uint32_t)reinterpret_cast<uintptr_t>(rr) & 15);
-            if (p.y) each([&](int c) { y[c].load_shared(ys + c * 32 * VEC * (int)sizeof(T)); }, [&](int c) { y[c].clear(); });
-            if (p.r) each([&](int c) { r[c].load_shared(rs + c * 32 * VEC * (int)sizeof(T)); }, [&](int c) { r[c].clear(); });
+            if (p.y) each([&](int c) { y[c].load_shared(ys + c * 32 * VEC * (int)sizeof(T)), own(y[c], c); }, [&](int c) { y[c].clear(); });
+            if (p.r) each([&](int c) { r[c].load_shared(rs + c * 32 * VEC * (int)sizeof(T)), own(r[c], c); }, [&](int c) { r[c].clear(); });
         }
         auto refill = [&]() { // all of the team's reads of the stage come before
             if (WARP) __syncwarp();
@@ -456,14 +489,15 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
             return team_sum<WARP>(sum2(s), sums + slot * 128) * p.inv_d;
         };
         auto centre = [&](float mean) {
-            if (full) {
-                const unsigned long long m = pack2f(-mean, -mean);
+            const unsigned long long m = pack2f(-mean, -mean);
 #pragma unroll
-                for (int j = 0; j < N; j += 2) unpack2f(add2(pack2f(u[j], u[j + 1]), m), u[j], u[j + 1]);
-            } else {
+            for (int j = 0; j < N; j += 2) unpack2f(add2(pack2f(u[j], u[j + 1]), m), u[j], u[j + 1]);
+            if (full) return;
 #pragma unroll
-                for (int j = 0; j < N; j++) u[j] = at(j / VEC) < d ? u[j] - mean : 0.f;
-            }
+            for (int c = 0; c < C; c++) // past the row's ends 0 again
+                if (!whole(c) || at(c) >= d + s)
+#pragma unroll
+                    for (int j = c * VEC; j < (c + 1) * VEC; j++) u[j] = valid(j) ? u[j] : 0.f;
         };
         auto scaled = [&](float scale, const float(&m)[N], const float(&b)[N]) { // u = scale u m + b
             const unsigned long long sc = pack2f(scale, scale);
@@ -473,8 +507,16 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
                 else unpack2f(fma2(mul2(pack2f(u[j], u[j + 1]), sc), pack2f(m[j], m[j + 1]), pack2f(b[j], b[j + 1])), u[j], u[j + 1]);
         };
         auto store = [&](T *to) {
-            to += at0;
-            each([&](int c) { store_values<T, VEC>(to + c * 32 * VEC, u + c * VEC); }, [](int) {});
+            T *const from = to + (at0 - s);
+            each([&](int c) {
+                if (full || whole(c)) {
+                    store_values<T, VEC>(from + c * 32 * VEC, u + c * VEC);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                        if (valid(c * VEC + j)) to[index(c * VEC + j)] = from_f32<T>(u[c * VEC + j]);
+                }
+            }, [](int) {});
         };
         if (p.y) {
 #pragma unroll
@@ -631,18 +673,25 @@ template <typename T, int VEC> __global__ void __launch_bounds__(1024) residual_
     });
 }
 
-template <typename T, int VEC, bool WARP, bool PLAIN> cudaError_t launch_walk(const ResidualNormParams &p, int sm_count, cudaStream_t stream) {
-    const auto kernel = residual_norm_walk_kernel<T, VEC, WARP, PLAIN>;
-    const int threads = WARP ? 32 : (p.d + N * 32 - 1) / (N * 32) * 32, teams = WARP ? MAX_TEAMS : 1;
-    const int stage = teams * walk_operand_bytes<VEC>(p.d * (int)sizeof(T)) * ((p.r != nullptr) + (p.y != nullptr));
+template <typename T, int VEC, bool WARP, bool PLAIN, bool SHIFT> cudaError_t launch_walk(const ResidualNormParams &p, int period, int sm_count, cudaStream_t stream) {
+    const auto kernel = residual_norm_walk_kernel<T, VEC, WARP, PLAIN, SHIFT>;
+    const int threads = WARP ? 32 : (p.d + (SHIFT ? VEC - 1 : 0) + N * 32 - 1) / (N * 32) * 32, teams = WARP ? MAX_TEAMS : 1;
+    const int stage = teams * walk_operand_bytes<(VEC > 1 && !SHIFT)>(p.d * (int)sizeof(T)) * ((p.r != nullptr) + (p.y != nullptr));
     const int per_sm = WALK_THREADS<PLAIN> / (threads * teams);
     const int stages = std::max(2, std::min(MAX_STAGES, WALK_SMEM / per_sm / stage));
     static SmemAttr attr;
     cudaError_t e = attr.ensure(kernel, (size_t)WALK_SMEM);
     if (e != cudaSuccess) return e;
-    const long long walkers = (long long)per_sm * sm_count * teams, share = (p.rows + walkers - 1) / walkers;
-    const long long used = (p.rows + share - 1) / share;
-    return launch_pdl(kernel, dim3((unsigned)((used + teams - 1) / teams)), dim3(threads, teams), (size_t)stages * stage, stream, p, (int)share, stages);
+    const long long rows = (p.rows + period - 1) / period; // of a kind
+    const long long walkers = std::max(1, per_sm * sm_count * teams / period), share = (rows + walkers - 1) / walkers;
+    const long long used = (rows + share - 1) / share * period;
+    return launch_pdl(kernel, dim3((unsigned)((used + teams - 1) / teams)), dim3(threads, teams), (size_t)stages * stage, stream, p, (int)share, stages, period);
+}
+
+template <typename T, int VEC, bool SHIFT> cudaError_t launch_walks(const ResidualNormParams &p, bool plain, int period, int sm_count, cudaStream_t stream) {
+    if (p.d + (SHIFT ? VEC - 1 : 0) <= 32 * N)
+        return plain ? launch_walk<T, VEC, true, true, SHIFT>(p, period, sm_count, stream) : launch_walk<T, VEC, true, false, SHIFT>(p, period, sm_count, stream);
+    return plain ? launch_walk<T, VEC, false, true, SHIFT>(p, period, sm_count, stream) : launch_walk<T, VEC, false, false, SHIFT>(p, period, sm_count, stream);
 }
 
 template <typename T, int VEC, int C, bool EARLY> cudaError_t launch_row(const ResidualNormParams &p, cudaStream_t stream) {
@@ -653,23 +702,40 @@ template <typename T, int VEC, int C, bool EARLY> cudaError_t launch_row(const R
 // a row fewer than there are warps to walk: they have one round of loads, where a team that stays asks for its constants first.
 // bf16, d = 2560, rms both sides: 77 rows 3.4 us a CTA each, 3.9 walked; 300 rows 4.7 and 4.0; 1500 rows 13.8 and 8.3.
 // f32, d = 384, 1500 rows: 3.9 and 4.7.
-template <typename T, int VEC> cudaError_t launch_t(const ResidualNormParams &p, int sm_count, cudaStream_t stream) {
-    constexpr int EARLY_C = VEC == 1 ? 4 : 1, WAVE = VEC == 1 ? 1024 : VEC == 4 ? 1344 : 704;
+template <typename T, int VEC> cudaError_t launch_t(const ResidualNormParams &p, int period, int sm_count, cudaStream_t stream) {
+    constexpr int EARLY_C = VEC == 1 ? 4 : 1, WAVE = VEC == 1 ? 1024 : VEC == 4 ? 1344 : 704, WORD = 16 / (int)sizeof(T);
     const int threads = (p.d + 32 * VEC * EARLY_C - 1) / (32 * VEC * EARLY_C) * 32;
     const bool few = p.rows <= (long long)sm_count * (WAVE / threads) || (p.d <= 32 * N && p.rows <= 2 * MAX_TEAMS * sm_count);
     if (p.d <= 4096 && (few || p.d < MIN_WALK_D)) return launch_row<T, VEC, EARLY_C, true>(p, stream);
     const bool plain = p.post.kind != RT_NORM_LAYER && p.pre.kind != RT_NORM_LAYER && !p.post.bias && !p.pre.bias;
-    if (p.d <= 32 * N) return plain ? launch_walk<T, VEC, true, true>(p, sm_count, stream) : launch_walk<T, VEC, true, false>(p, sm_count, stream);
-    if (plain && p.d <= WALK_THREADS<true> * N) return launch_walk<T, VEC, false, true>(p, sm_count, stream);
-    if (p.d <= WALK_THREADS<false> * N) return launch_walk<T, VEC, false, false>(p, sm_count, stream);
+    const int longest = (plain ? WALK_THREADS<true> : WALK_THREADS<false>) * N;
+    // operands that lie alike go by 16-byte words (8192 bf16 rows of 2561: 53 us, 71 value by value; 52000 rows of 383: 67 and 67, with
+    // means and biases 93 and 102)
+    if constexpr (VEC == 1)
+        if (period && p.d + WORD - 1 <= longest) return launch_walks<T, WORD, true>(p, plain, period, sm_count, stream);
+    if (p.d <= longest) return launch_walks<T, VEC, false>(p, plain, 1, sm_count, stream);
     // longer rows, 32 values a thread in registers while 512 threads hold them (2048 bf16 rows of 10240: 51 us, 103 with the loops;
     // value by value, rows of 9001, 282 and 128)
     if constexpr (VEC > 1)
         if (p.d <= 512 * 32) return launch_row<T, VEC, 32 / VEC, false>(p, stream);
     return launch_pdl(residual_norm_loop_kernel<T, VEC>, dim3(p.rows), dim3(1024), 0, stream, p);
 }
+// vec: every access on a 16-byte boundary; else the period in which rows lie the same way, or 0 where operands differ in that
 template <typename T> cudaError_t launch_t(const ResidualNormParams &p, bool vec, int sm_count, cudaStream_t stream) {
-    return vec ? launch_t<T, 16 / (int)sizeof(T)>(p, sm_count, stream) : launch_t<T, 1>(p, sm_count, stream);
+    if (vec) return launch_t<T, 16 / (int)sizeof(T)>(p, 1, sm_count, stream);
+    uintptr_t base = 0;
+    long long pitch = 0;
+    int period = 0;
+    const std::pair<const void *, long long> operands[] = {{p.y, p.y_ld}, {p.r, p.r_ld}, {p.h, p.h_ld}, {p.x, p.x_ld}};
+    for (const auto &o : operands) {
+        if (!o.first) continue;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(o.first) % 16;
+        const long long step = o.second * (long long)sizeof(T) % 16;
+        if (period && (at != base || step != pitch)) return launch_t<T, 1>(p, 0, sm_count, stream);
+        base = at, pitch = step, period = 1;
+    }
+    while (pitch * period % 16) period *= 2;
+    return launch_t<T, 1>(p, period, sm_count, stream);
 }
 
 } // namespace

@@ -749,3 +749,38 @@ def test_vocabularies_that_a_cluster_s_ctas_share(dt, vocab, gpu):
             v[1, [0, vocab - 1]] = 1.0
         tokens = [0] * rows if rows != 2 else None
         lp_check(v, tokens, top, gpu, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+def test_many_rows_off_the_16_byte_boundary(dt, gpu):
+    """Every way rows can lie: all operands shifted alike (each shift, constant or changing from row to row), and each differently."""
+    rng, rows, lib = np.random.default_rng(61), 700, _lib.load()
+    size = 4 if dt == F32 else 2
+    store = {F16: lambda v: v.astype(np.float16), F32: lambda v: v,
+             BF16: lambda v: (v.view(np.uint32) >> 16).astype(np.uint16)}[dt]
+    back = {F16: lambda b: b.astype(np.float32), F32: lambda b: b,
+            BF16: lambda b: (b.astype(np.uint32) << 16).view(np.float32)}[dt]
+    for d, ld, shifts in ((1001, 1001, (0, 0, 0, 0)), (1002, 1002, (0, 0, 0, 0)), (1004, 1004, (1, 1, 1, 1)), (1000, 1000, (3, 3, 3, 3)), (1000, 1008, (7, 7, 7, 7)), (513, 520, (8, 0, 16, 24)),
+                          (1001, 1001, (0, 1, 0, 0)), (1001, 1003, (0, 0, 5, 0)), (2047, 2047, (5, 5, 5, 5)), (1500, 1501, (2, 2, 2, 10))):
+        mats = [round_to(dt, rng.standard_normal(rows * ld + 40, dtype=np.float32)) for _ in range(2)] + [np.zeros(rows * ld + 40, np.float32)] * 2
+        bufs = [device_array(gpu, store(m)) for m in mats]
+        for kind in (_lib.RT_NORM_RMS, _lib.RT_NORM_LAYER):
+            w = [round_to(dt, (1 + 0.3 * rng.standard_normal(d)).astype(np.float32)) for _ in range(2)]
+            wb = [device_array(gpu, store(v)) for v in w]
+            p = _lib.rt_residual_norm()
+            p.dt, p.residual_scale, p.block_scale, p.rows, p.d = int(dt), 0.5, 2.0, rows, d
+            p.residual, p.block, p.h, p.x = (b.ptr + size * s for b, s in zip(bufs, shifts))
+            p.residual_ld = p.block_ld = p.h_ld = p.x_ld = ld
+            for n, b in ((p.post, wb[0]), (p.pre, wb[1])):
+                n.kind, n.dt, n.eps, n.weight = kind, int(dt), 1e-5, b.ptr
+            _lib.check(lib.rt_residual_norm_launch(gpu._h, ctypes.byref(p), None))
+            at = [(s + np.arange(rows)[:, None] * ld + np.arange(d)[None, :]).reshape(-1) for s in shifts]
+            r, y = (m[a].reshape(rows, d).astype(np.float64) for m, a in zip(mats[:2], at))
+            name, eps = "rms" if kind == _lib.RT_NORM_RMS else "layer", np.float64(np.float32(1e-5))
+            truths = norm_truth(r, y, None, (name, w[0].astype(np.float64), 0.0, eps), (name, w[1].astype(np.float64), 0.0, eps), 0.5, 2.0)
+            for b, a, t in zip(bufs[2:], at[2:], truths):
+                got = read_back(gpu, b, store(mats[2]))
+                rest = np.ones(got.size, bool)
+                rest[a] = False
+                assert not got[rest].any() and np.all(close(back(got[a]).reshape(rows, d), t, dt)), (d, ld, shifts, name)
