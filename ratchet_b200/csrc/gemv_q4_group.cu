@@ -17,12 +17,14 @@
 //    points, a word a group (read from global memory by the lanes that need them they would be more requests than the codes).
 //  * f32 sums of a group times s, added in f32 over steps, warps and CTAs of the cluster in a fixed order.
 //
-// One vector, 51200 rows of 2560: 15.7 us with groups of 128 (4.4 TB/s), 17.2 of 64, 19.1 of 32; 2560 x 2560 3.8, the launch and two
-// trips to memory; 16 vectors 25.4 / 31 / 48: the epilogue of a group (FMAs by vectors) and the masking bound those.  A CUDA-core
-// product of the same layout took 5 to 80 times as long (2560 x 10240 with 5 vectors: 841 us against 10.0).
+// One vector, 51200 rows of 2560: 16.1 us with groups of 128 (4.3 TB/s), 17.1 of 64, 18.8 of 32; 2560 x 2560 3.8, the launch and two
+// trips to memory; 16 vectors 23.9 / 29 / 47: the epilogue of a group (FMAs by vectors, in pairs) and the masking bound
+// those.  A CUDA-core
+// product of the same layout took 5 to 80 times as long (2560 x 10240 with 5 vectors: 841 us against 9.8).
 #include <algorithm>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "kernels.hpp"
 
 namespace rt {
@@ -334,11 +336,9 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     }
     __syncthreads();
 
-    float acc[P][4];
+    unsigned long long sums[P][2]; // of the lane's two columns, a pair for row g and one for row g + 8
 #pragma unroll
-    for (int v = 0; v < P; v++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[v][j] = 0.f;
+    for (int v = 0; v < P; v++) sums[v][0] = sums[v][1] = 0;
     // B operand: the lane's column is vector g (SPREAD; columns without a vector repeat the last one and are not stored), or vector
     // g % VP of group g / VP, zero where the lane's values are of another group
     const int own_group = SPREAD ? 0 : t * G / 4;
@@ -355,24 +355,20 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     uint4 b0[4]; // without SPREAD: the step's B operands (lanes that are not on keep zeros)
 #pragma unroll
     for (int j = 0; j < 4; j++) b0[j] = make_uint4(0, 0, 0, 0);
-    auto pair_at = [](const float *at, float (&v)[2]) {
-        if (NVS == 1) {
-            v[0] = v[1] = *at;
-        } else {
-            const float2 f = *reinterpret_cast<const float2 *>(at);
-            v[0] = f.x, v[1] = f.y;
-        }
+    auto pair_at = [](const float *at) {
+        if (NVS == 1) return pack2f(*at, *at);
+        return *reinterpret_cast<const unsigned long long *>(at);
     };
+    const unsigned long long k16 = pack2f(16.f, 16.f), k20 = pack2f(1048576.f, 1048576.f);
     auto do_step = [&](uint32_t (&c)[2][4]) {
         if (!SPREAD && on) {
 #pragma unroll
             for (int j = 0; j < 4; j++) b0[j] = xb[j * NVS * 4];
         }
         if (MIX && G == 4) spread_words(c[0], t), spread_words(c[1], t);
-        float back[P][2];
+        unsigned long long back[P];
 #pragma unroll
-        for (int v = 0; v < P; v++)
-            if (BF16) pair_at(up_at + v * 8, back[v]);
+        for (int v = 0; v < P; v++) back[v] = BF16 ? pair_at(up_at + v * 8) : 0;
 #pragma unroll
         for (int grp = 0; grp < XS; grp++) { // words 4 grp / XS .. of one group; without SPREAD the lane's own group
             float d[2][P][4];
@@ -391,20 +387,19 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
             }
 #pragma unroll
             for (int v = 0; v < P; v++) {
-                float sx[2];
-                pair_at(xsum_at + grp * NVS + v * 8, sx);
+                const unsigned long long sx = pair_at(xsum_at + grp * NVS + v * 8);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const uint32_t e = sc[h * sc_half + grp];
                     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&e)); // s, z
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        float &to = acc[v][2 * h + j];
-                        const float n = fmaf(d[0][v][2 * h + j], 16.f, d[1][v][2 * h + j]); // 2^-20 times the sum of q x
-                        if (BF16) // s and the power of two together: neither alone may be taken to the sum
-                            to = fmaf(f.x * back[v][j], fmaf(n, 1048576.f, -f.y * sx[j]), to);
-                        else
-                            to = fmaf(-f.x * f.y, sx[j], fmaf(f.x * 1048576.f, n, to));
+                    unsigned long long &to = sums[v][h];
+                    // 2^-20 times the sum of q x
+                    const unsigned long long n = fma2(pack2f(d[0][v][2 * h], d[0][v][2 * h + 1]), k16, pack2f(d[1][v][2 * h], d[1][v][2 * h + 1]));
+                    if (BF16) { // s and the power of two together: neither alone may be taken to the sum
+                        to = fma2(mul2(pack2f(f.x, f.x), back[v]), fma2(n, k20, mul2(pack2f(-f.y, -f.y), sx)), to);
+                    } else {
+                        const float s20 = f.x * 1048576.f, sz = -f.x * f.y;
+                        to = fma2(pack2f(sz, sz), sx, fma2(pack2f(s20, s20), n, to));
                     }
                 }
             }
@@ -430,15 +425,18 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     float *const mine_at = part + (kpart * q.units + tile) * SLOT;
 #pragma unroll
     for (int v = 0; v < P; v++) {
+        float acc[4];
+        unpack2f(sums[v][0], acc[0], acc[1]);
+        unpack2f(sums[v][1], acc[2], acc[3]);
 #pragma unroll
         for (int j = 0; j < 4; j++) { // the groups of a vector are in lanes VP / 2 apart
-            if (!SPREAD && G == 4) acc[v][j] += __shfl_xor_sync(0xffffffffu, acc[v][j], 1);
-            if (!SPREAD && G >= 2) acc[v][j] += __shfl_xor_sync(0xffffffffu, acc[v][j], 2);
+            if (!SPREAD && G == 4) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], 1);
+            if (!SPREAD && G >= 2) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], 2);
         }
         const int vec = v * VP + 2 * t;
         float *const at = mine_at + vec * 16 + g;
-        if (2 * t < VP && vec < q.nv) at[0] = acc[v][0], at[8] = acc[v][2];
-        if (2 * t < VP && vec + 1 < q.nv) at[16] = acc[v][1], at[24] = acc[v][3];
+        if (2 * t < VP && vec < q.nv) at[0] = acc[0], at[8] = acc[2];
+        if (2 * t < VP && vec + 1 < q.nv) at[16] = acc[1], at[24] = acc[3];
     }
     __syncthreads();
     auto sum_of = [&](int e) {
