@@ -74,14 +74,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// 16 (8) bytes of codes where `on`; else the registers keep what they hold
-__device__ __forceinline__ void load_codes(uint32_t (&w)[4], const uint8_t *p, bool on) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}\n"
-                 : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(p), "r"((uint32_t)on));
+// 16 bytes of codes, or 8 here and 8 bytes 32 further on
+__device__ __forceinline__ void load_codes(uint32_t (&w)[4], const uint8_t *p) {
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
-__device__ __forceinline__ void load_codes_halves(uint32_t (&w)[4], const uint8_t *p, bool on) { // 8 bytes here, 8 bytes 32 further on
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.nc.v2.u32 {%0,%1}, [%4];\n\t@p ld.global.nc.v2.u32 {%2,%3}, [%4+32];\n\t}\n"
-                 : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]) : "l"(p), "r"((uint32_t)on));
+__device__ __forceinline__ void load_codes_halves(uint32_t (&w)[4], const uint8_t *p) {
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "l"(p + 32));
 }
 
 // Two bf16 values of a 32-bit word times `scale` (a power of two) as f16
@@ -174,29 +173,27 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
     const int first = rank * q.per_rank, n_steps = max(0, min(q.steps, first + q.per_rank) - first); // of this CTA
     const uint32_t row_bytes = (uint32_t)K >> 1;
 
-    // ---- the warp's rows and steps; the first codes.  Rows that are not the CTA's are not read: what their places of an MMA hold
-    // is finite and goes nowhere.  The last step of a row whose K is no multiple of 128 reads on into what lies behind it (the
-    // next row, or the scales); its scales and activations are 0.
+    // ---- the warp's rows and steps; the first codes.  Rows that are not the CTA's are its last one again, with scales of 0.  The last
+    // step of a row whose K is no multiple of 128 reads on into what lies behind it (the next row, or the scales); its scales and
+    // activations are 0.
     const int kpart = q.parts > 1 ? warp % q.parts : 0, tile = q.parts > 1 ? warp / q.parts : warp;
     const int begin = min(n_steps, kpart * q.per_part), end = min(n_steps, begin + q.per_part); // within this CTA's steps
-    const uint8_t *code0 = (const uint8_t *)p.lhs + (lhs_row + tile * unit + g) * row_bytes + (uint32_t)(first + begin) * (STEP / 2) + t * (MIX ? 8 : 16);
-    const long long half_bytes = (long long)(q.pair ? ff : 8) * row_bytes;
-    const bool have[2] = {tile * unit + g < have_rows, tile * unit + g + (q.pair ? 0 : 8) < have_rows};
+    const int row0 = min(tile * unit + g, have_rows - 1), row1 = q.pair ? row0 + ff : min(tile * unit + g + 8, have_rows - 1);
+    const uint8_t *const codes = (const uint8_t *)p.lhs + (uint32_t)(first + begin) * (STEP / 2) + t * (MIX ? 8 : 16);
+    const uint8_t *code0 = codes + (lhs_row + row0) * row_bytes;
+    const long long half_bytes = (long long)(row1 - row0) * row_bytes;
     uint32_t code[AHEAD][2][4];
-#pragma unroll
-    for (int a = 0; a < AHEAD; a++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) code[a][0][k] = code[a][1][k] = 0;
-    auto load = [&](uint32_t (&c)[2][4], const uint8_t *at, bool in) {
+    auto load = [&](uint32_t (&c)[2][4], const uint8_t *at) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const uint8_t *from = at + (h ? half_bytes : 0);
-            if (MIX) load_codes_halves(c[h], from, have[h] && in);
-            else load_codes(c[h], from, have[h] && in);
+            if (MIX) load_codes_halves(c[h], from);
+            else load_codes(c[h], from);
         }
     };
 #pragma unroll
-    for (int a = 0; a < AHEAD; a++) load(code[a], code0 + a * (STEP / 2), begin + a < end);
+    for (int a = 0; a < AHEAD; a++)
+        if (begin + a < end) load(code[a], code0 + a * (STEP / 2));
 
     // ---- scales of the rows' groups in this K range, 0 (a group that adds nothing) past K: four groups of a row at a time where
     // their number allows it, FOURS of a thread asked for together, the first ones before it waits for the stream predecessor
@@ -415,7 +412,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32) q4_group_gemv_kernel(const __g
         for (int a = 0; a < AHEAD; a++) {
             if (step + a >= end) break;
             do_step(code[a]);
-            load(code[a], code0 + a * (STEP / 2), step + a + AHEAD < end);
+            if (step + a + AHEAD < end) load(code[a], code0 + a * (STEP / 2));
         }
         code0 += AHEAD * (STEP / 2);
     }
