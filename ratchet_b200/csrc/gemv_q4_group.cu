@@ -17,10 +17,9 @@
 //    points, a word a group (read from global memory by the lanes that need them they would be more requests than the codes).
 //  * f32 sums of a group times s, added in f32 over steps, warps and CTAs of the cluster in a fixed order.
 //
-// One vector, 51200 rows of 2560: 16.1 us with groups of 128 (4.3 TB/s), 17.1 of 64, 18.8 of 32; 2560 x 2560 3.8, the launch and two
-// trips to memory; 16 vectors 23.9 / 29 / 47: the epilogue of a group (FMAs by vectors, in pairs) and the masking bound
-// those.  A CUDA-core
-// product of the same layout took 5 to 80 times as long (2560 x 10240 with 5 vectors: 841 us against 9.8).
+// One vector, 51200 rows of 2560: 15.2 us with groups of 128 (4.5 TB/s), 16.6 of 64, 18.2 of 32; 2560 x 2560 3.7, the launch and two
+// trips to memory; 16 vectors 23.5 / 29 / 46: the epilogue of a group (FMAs by vectors, in pairs) and the masking bound those.  A
+// CUDA-core product of the same layout took 5 to 80 times as long (2560 x 10240 with 5 vectors: 841 us against 9.7).
 #include <algorithm>
 
 #include "common.cuh"
