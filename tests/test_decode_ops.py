@@ -784,3 +784,58 @@ def test_many_rows_off_the_16_byte_boundary(dt, gpu):
                 rest = np.ones(got.size, bool)
                 rest[a] = False
                 assert not got[rest].any() and np.all(close(back(got[a]).reshape(rows, d), t, dt)), (d, ld, shifts, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("d,rows", [(520, 3), (1000, 900), (1001, 900), (40, 4000)])
+def test_a_block_without_a_residual_and_x_without_h(d, rows, dt, gpu):
+    rng, lib = np.random.default_rng(71), _lib.load()
+    np_dt = np.float16 if dt == F16 else np.float32
+    r, y = (round_to(dt, rng.standard_normal((rows, d), dtype=np.float32)) for _ in range(2))
+    w, w_t = norm_weights("rms", d, dt, rng)
+    rb_, yb, wb, hb, xb = (device_array(gpu, np.ascontiguousarray(v.astype(np_dt))) for v in (r, y, w[0], 0 * r, 0 * r))
+    for residual in (True, False):
+        p = _lib.rt_residual_norm()
+        p.dt, p.residual_scale, p.block_scale, p.rows, p.d = int(dt), 1.5, -0.5, rows, d
+        p.residual, p.block, p.h, p.x = rb_.ptr if residual else None, yb.ptr, None if residual else hb.ptr, xb.ptr
+        p.residual_ld = p.block_ld = p.h_ld = p.x_ld = d
+        for n in (p.post, p.pre):
+            n.kind, n.dt, n.eps, n.weight = _lib.RT_NORM_RMS, int(dt), w[2], wb.ptr
+        _lib.check(lib.rt_residual_norm_launch(gpu._h, ctypes.byref(p), None))
+        th, tx = norm_truth(r.astype(np.float64) if residual else None, y.astype(np.float64), None, w_t, w_t, 1.5, -0.5)
+        assert np.all(close(read_back(gpu, xb, r.astype(np_dt)).astype(np.float32), tx, dt)), residual
+        if not residual:
+            assert np.all(close(read_back(gpu, hb, r.astype(np_dt)).astype(np.float32), th, dt))
+
+
+@pytest.mark.gpu
+def test_rows_whose_offsets_pass_32_bits(gpu):
+    """Windows of a matrix of 2.4 thousand million values: the first and the last rows."""
+    import torch
+    rows, ld, lib = 1200, 2_000_001, _lib.load()
+    big = torch.zeros(rows * ld, dtype=torch.half, device="cuda")
+    m, rng = big.view(rows, ld), np.random.default_rng(72)
+    for d, at in ((1001, 5), (1000, 8)):
+        r = round_to(F16, rng.standard_normal((rows, d), dtype=np.float32))
+        m[:, at:at + d] = torch.from_numpy(r).half().cuda()
+        w = torch.ones(d, dtype=torch.half, device="cuda")
+        torch.cuda.synchronize()
+        p = _lib.rt_residual_norm()
+        p.dt, p.residual_scale, p.rows, p.d, p.residual_ld, p.x_ld = _lib.RT_F16, 1.0, rows, d, ld, ld
+        p.residual, p.x = big.data_ptr() + 2 * at, big.data_ptr() + 2 * (at + 4096)
+        p.pre.kind, p.pre.dt, p.pre.eps, p.pre.weight = _lib.RT_NORM_RMS, _lib.RT_F16, 1e-5, w.data_ptr()
+        _lib.check(lib.rt_residual_norm_launch(gpu._h, ctypes.byref(p), None))
+        gpu.sync()
+        want = normed(r.astype(np.float64), 0 * r.astype(np.float64), "rms", 1.0, 0.0, np.float64(np.float32(1e-5)))
+        assert np.all(close(m[:, at + 4096:at + 4096 + d].float().cpu().numpy(), want, F16))
+    ent, ids, tops = torch.zeros(rows, device="cuda"), torch.zeros(rows, 3, dtype=torch.int32, device="cuda"), torch.zeros(rows, 3, device="cuda")
+    q = _lib.rt_log_probs()
+    q.dt, q.top, q.rows, q.vocab, q.ld, q.logits = _lib.RT_F16, 3, rows, 1000, ld, big.data_ptr() + 16
+    q.entropy, q.top_ids, q.top_log_prob = ent.data_ptr(), ids.data_ptr(), tops.data_ptr()
+    torch.cuda.synchronize()
+    _lib.check(lib.rt_log_probs_launch(gpu._h, ctypes.byref(q), None))
+    gpu.sync()
+    logp, want, order, loss, ent_loss = lp_truth(r)
+    assert np.array_equal(ids.cpu().numpy(), order[:, :3]) and np.all(np.abs(ent.cpu().numpy() - want) <= ent_loss + 4 * E24 * np.abs(want))
+    assert np.all(np.abs(tops.cpu().numpy() - np.take_along_axis(logp, order[:, :3], 1)) <= loss[:, None] + 4 * E24 * 20)

@@ -450,3 +450,42 @@ def test_the_gemv_on_two_streams_and_in_a_replayed_graph(gpu):
         for case in cases:
             right(case)
     del graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 12, 40, 130])
+def test_a_weight_per_batch_with_any_number_of_rows(rows, gpu):
+    w, wv = weight(G64, (3, 130, 320), 51)
+    x = activations(F16, (3, rows, 320), 52)
+    y = np.einsum("bmk,bnk->bnm", wv, x.astype(np.float64))
+    e = np.stack([error_bound(F16, wv[b], x[b].astype(np.float64), y[b], rounded_weights=True) for b in range(3)])
+    got = w.to(gpu).gemm(Tensor.from_data(x, gpu, F16), None, False, True, True).resolve().to(Device.CPU).to_f32()
+    assert np.all(np.abs(got - y) <= e)
+
+
+@pytest.mark.gpu
+def test_a_weight_whose_offsets_pass_32_bits(gpu):
+    """1.7 million rows of 2560: 4.4 thousand million values; rows from all over it."""
+    import torch
+    m, k = 1_700_003, 2560
+    lib, parts = _lib.load(), G128.segments(m * k)
+    buf = torch.zeros(G128.nbytes(m * k), dtype=torch.uint8, device="cuda")
+    codes, scales, zeros = (buf[at:at + n] for (at, _), n in zip(parts, (m * k // 2, m * k // 64, m * k // 128)))
+    gen = torch.Generator(device="cuda").manual_seed(53)
+    codes.random_(0, 256, generator=gen), zeros.random_(0, 16, generator=gen)
+    scales.view(torch.half).uniform_(0.005, 0.02, generator=gen)
+    pick = np.unique(np.concatenate([np.arange(20), np.arange(m - 20, m), np.random.default_rng(54).integers(0, m, 200), [m * 5 // 8 + i for i in range(20)]]))
+    at = torch.from_numpy(pick).cuda()
+    q = codes.view(m, k // 2)[at].cpu().numpy()
+    wv = values(G128, np.stack([q & 15, q >> 4], -1).reshape(len(pick), k), scales.view(torch.half).view(m, k // 128)[at].cpu().numpy(), zeros.view(m, k // 128)[at].cpu().numpy())
+    for rows in (1, 4):
+        x = activations(F16, (1, rows, k), 55)
+        xg = torch.from_numpy(x).half().cuda()
+        out = torch.zeros(rows, m, dtype=torch.half, device="cuda")
+        plan = gpu.plan_for(Linear(Tensor((m, k), G128, gpu)).schedule(Tensor((1, rows, k), F16, gpu)).op.desc)
+        torch.cuda.synchronize()
+        _lib.check(lib.rt_matmul_launch(plan, buf.data_ptr(), xg.data_ptr(), None, out.data_ptr(), None))
+        gpu.sync()
+        y = x[0].astype(np.float64) @ wv.T
+        kernel = lib.rt_plan_kernel(plan).decode()
+        assert "q4_group_gemv" in kernel and np.all(np.abs(out[:, at].double().cpu().numpy() - y) <= error_bound(F16, wv, x[0].astype(np.float64), y)), kernel
