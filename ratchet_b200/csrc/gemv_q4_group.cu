@@ -31,7 +31,7 @@ namespace rt {
 namespace {
 
 constexpr int STEP = 128; // values of k per warp and step
-constexpr int MAX_WARPS = 24; // of a CTA: 80 registers a thread
+constexpr int MAX_WARPS = 24; // of a CTA: 80 registers a thread (51200 x 2560, one vector: 15.2 us, with 32 warps at 64 registers and two steps ahead 17.3)
 
 struct Q4GroupParams {
     MatmulParams p;
