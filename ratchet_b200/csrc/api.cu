@@ -1320,6 +1320,20 @@ static rt_status dispatch_node(rt_executable *exe, size_t i, cudaStream_t st) {
     return launch_node(n.plan, n.lhs, n.rhs, n.bias, n.out, (void *)st, &n.opts, &exe->scratch[i]);
 }
 
+// checked descriptions
+static rt_status launch_norm(rt_device *dev, const rt_residual_norm &op, cudaStream_t st) {
+    if (op.rows == 0) return RT_OK;
+    CUDA_TRY(cudaSetDevice(dev->ordinal));
+    CUDA_TRY(launch_residual_norm(op, dev->sm_count, st));
+    return RT_OK;
+}
+static rt_status launch_probs(rt_device *dev, const rt_log_probs &op, cudaStream_t st) {
+    if (op.rows == 0) return RT_OK;
+    CUDA_TRY(cudaSetDevice(dev->ordinal));
+    CUDA_TRY(launch_log_probs(op, dev->sm_count, st));
+    return RT_OK;
+}
+
 static rt_status dispatch_nodes(rt_executable *exe, cudaStream_t st) {
     if (exe->steps.empty()) {
         for (size_t i = 0; i < exe->nodes.size(); i++)
@@ -1329,8 +1343,8 @@ static rt_status dispatch_nodes(rt_executable *exe, cudaStream_t st) {
     size_t node = 0;
     for (const rt_step &step : exe->steps) {
         const rt_status s = step.kind == RT_STEP_MATMUL          ? dispatch_node(exe, node++, st)
-                            : step.kind == RT_STEP_RESIDUAL_NORM ? rt_residual_norm_launch(exe->dev, &step.norm, (void *)st)
-                                                                 : rt_log_probs_launch(exe->dev, &step.log_probs, (void *)st);
+                            : step.kind == RT_STEP_RESIDUAL_NORM ? launch_norm(exe->dev, step.norm, st)
+                                                                 : launch_probs(exe->dev, step.log_probs, st);
         if (s != RT_OK) return s;
     }
     return RT_OK;
@@ -1626,10 +1640,8 @@ rt_status rt_residual_norm_check(const rt_residual_norm *op) {
 
 rt_status rt_residual_norm_launch(rt_device *dev, const rt_residual_norm *op, void *stream) {
     if (!dev) return fail(RT_ERR_ARG, "rt_residual_norm: null device");
-    if (rt_status s = rt_residual_norm_check(op); s != RT_OK || op->rows == 0) return s;
-    CUDA_TRY(cudaSetDevice(dev->ordinal));
-    CUDA_TRY(launch_residual_norm(*op, dev->sm_count, stream ? (cudaStream_t)stream : dev->stream));
-    return RT_OK;
+    if (rt_status s = rt_residual_norm_check(op); s != RT_OK) return s;
+    return launch_norm(dev, *op, stream ? (cudaStream_t)stream : dev->stream);
 }
 
 rt_status rt_log_probs_check(const rt_log_probs *op) {
@@ -1640,10 +1652,8 @@ rt_status rt_log_probs_check(const rt_log_probs *op) {
 
 rt_status rt_log_probs_launch(rt_device *dev, const rt_log_probs *op, void *stream) {
     if (!dev) return fail(RT_ERR_ARG, "rt_log_probs: null device");
-    if (rt_status s = rt_log_probs_check(op); s != RT_OK || op->rows == 0) return s;
-    CUDA_TRY(cudaSetDevice(dev->ordinal));
-    CUDA_TRY(launch_log_probs(*op, dev->sm_count, stream ? (cudaStream_t)stream : dev->stream));
-    return RT_OK;
+    if (rt_status s = rt_log_probs_check(op); s != RT_OK) return s;
+    return launch_probs(dev, *op, stream ? (cudaStream_t)stream : dev->stream);
 }
 
 int32_t rt_executable_launches(const rt_executable *exe) { return exe ? exe->launches : 0; }

@@ -37,16 +37,16 @@ bool overlap(const Rows &a, const Rows &b) {
 Status arg(const std::string &m) { return Status::Err(RT_ERR_ARG, m); }
 
 Status check_norm(const rt_norm &n, rt_dtype dt, const char *which) {
-    const std::string name = std::string("rt_residual_norm: ") + which;
+    auto name = [&]() { return std::string("rt_residual_norm: ") + which; };
     if (n.kind == RT_NORM_NONE) return Status::Ok();
-    if (n.kind != RT_NORM_RMS && n.kind != RT_NORM_LAYER) return arg(name + ": invalid norm kind");
-    if (!(n.eps >= 0.f) || std::isinf(n.eps)) return arg(name + ": eps must be finite and not negative");
+    if (n.kind != RT_NORM_RMS && n.kind != RT_NORM_LAYER) return arg(name() + ": invalid norm kind");
+    if (!(n.eps >= 0.f) || std::isinf(n.eps)) return arg(name() + ": eps must be finite and not negative");
     if (n.weight || n.bias) {
         if (n.dt != RT_F32 && n.dt != dt)
-            return Status::Err(RT_ERR_DTYPE, name + ": weight and bias are F32 or of the activations' type, not " + (dtype_valid(n.dt) ? dtype_name(n.dt) : "?"));
-        if (!aligned_to(n.weight, dtype_size(n.dt)) || !aligned_to(n.bias, dtype_size(n.dt))) return arg(name + ": misaligned weight or bias");
+            return Status::Err(RT_ERR_DTYPE, name() + ": weight and bias are F32 or of the activations' type, not " + (dtype_valid(n.dt) ? dtype_name(n.dt) : "?"));
+        if (!aligned_to(n.weight, dtype_size(n.dt)) || !aligned_to(n.bias, dtype_size(n.dt))) return arg(name() + ": misaligned weight or bias");
     }
-    if (n.bias && n.kind != RT_NORM_LAYER) return arg(name + ": only a layer norm takes a bias");
+    if (n.bias && n.kind != RT_NORM_LAYER) return arg(name() + ": only a layer norm takes a bias");
     return Status::Ok();
 }
 
