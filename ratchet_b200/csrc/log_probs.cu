@@ -277,11 +277,11 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
     };
 #pragma unroll
     for (int k = 0; k < GROUPS; k++) ask(k);
-    auto rank_group = [&](float m, int at) {
-        const bool first = !(m <= best);
-        second = first ? best : !(m <= second) ? m : second;
-        best = first ? m : best;
-        best_at = first ? at : best_at;
+    auto rank_group = [&](float m, int at) { // (the maxima keep a NaN, the minimum leaves it behind for the other: NaN is the largest)
+        const float larger = max_nan(best, m);
+        best_at = __float_as_uint(larger) != __float_as_uint(best) ? at : best_at; // (max.NaN has one NaN only)
+        second = max_nan(second, fminf(best, m));
+        best = larger;
     };
     int left = my_chunks, part = 0;
     for (; left >= GROUP; left -= GROUP, part = (part + 1) % GROUPS) {

@@ -1,0 +1,62 @@
+"""Log probabilities and residual norms where they can go wrong: what is not finite, masks, values far from zero, very long rows."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from ratchet_b200 import Device, DType, LayerNorm, RatchetError, ResidualNorm, RMSNorm, Tensor
+from ratchet_b200 import _lib
+from test_decode_ops import E24, close, lp_check, lp_truth, norm_truth
+from util import round_to
+
+F16, BF16, F32 = DType.F16, DType.BF16, DType.F32
+LOWEST = {F16: -65504.0, BF16: -3.3895313892515355e38, F32: -3.4028234663852886e38}
+HALF = {F16: 2.0**-11, BF16: 2.0**-8, F32: 2.0**-24}
+
+
+def run_log_probs(v, tokens, top, gpu, dt):
+    lp = Tensor.from_data(v, gpu, dt).log_probs(Tensor.from_data(np.asarray(tokens, np.int32), gpu), top)
+    lp.entropy.resolve()
+    return [None if t is None else t.resolve().to(Device.CPU).to_numpy() for t in lp]
+
+
+def order_with_nan(v):
+    """Each row's ids, NaN above all, equal values (and NaNs) by lower id."""
+    nan = np.isnan(v)
+    ids = np.broadcast_to(np.arange(v.shape[1]), v.shape)
+    return np.lexsort((ids, -np.where(nan, 0.0, v.astype(np.float64)), ~nan), axis=-1)
+
+
+# ------------------------------------------------------------------------------------------------ NaN
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(1, 51865), (16, 51865), (400, 20003), (1, 160000), (2, 300001)])
+def test_a_nan_anywhere_makes_its_row_nan_and_comes_first(rows, vocab, dt, gpu):
+    """A NaN in the first, a middle and the last value a thread takes, in the partial chunks at both ends, in every CTA's share of a
+    long row, beside +inf, alone among -inf, and two and forty of them; rows without one keep their answers."""
+    rng, top = np.random.default_rng(81), 20
+    v = round_to(dt, rng.standard_normal((rows, vocab), dtype=np.float32))
+    tokens = rng.integers(0, vocab, rows)
+    places = [[0], [5], [vocab - 1], [vocab - 9], [vocab // 2], [4096], [vocab // 8 - 1], [vocab // 8 + 3], [vocab * 7 // 8], [17, 17 + 8192], [3, vocab - 2],
+              [8 * 513], list(range(40, vocab, vocab // 40))[:40]]
+    clean = run_log_probs(v, tokens, top, gpu, dt)
+    for k in range(0, len(places) + 2, max(1, rows - 1)):
+        bad, hit = v.copy(), []
+        for r in range(0 if rows == 1 else 1, rows):  # with several rows, the first stays as it is
+            case = k + r - (rows > 1)
+            if case >= len(places) + 2:
+                break
+            if case < len(places):
+                bad[r, places[case]] = np.nan
+            elif case == len(places):
+                bad[r, 700], bad[r, vocab - 700] = np.inf, np.nan
+            else:
+                bad[r], bad[r, vocab // 3] = -np.inf, np.nan
+            hit.append(r)
+        got = run_log_probs(bad, tokens, top, gpu, dt)
+        rest = np.setdiff1d(np.arange(rows), hit)
+        for c, g in zip(clean, got):
+            assert np.array_equal(c[rest], g[rest])
+        assert np.isnan(got[0][hit]).all() and np.isnan(got[1][hit]).all() and np.isnan(got[3][hit]).all(), (k, hit)
+        assert np.array_equal(got[2][hit], order_with_nan(bad[hit])[:, :top]), k
