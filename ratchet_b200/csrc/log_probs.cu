@@ -34,13 +34,14 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float NO_REFERENCE = -1e38f, LOWEST = -1e38f; // values below LOWEST count as it: their t is finite and 2^t is 0
 using Order = unsigned long long;
 
-// larger value = larger word; -0 counts as +0, NaN as the largest; 0 is no value's word
+// larger value = larger word; -0 counts as +0, NaN as the largest; 0 is no value's word, nor is the largest one: a token's Order lies
+// below ~0
 __device__ __forceinline__ uint32_t order_bits(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
-    return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return v != v ? 0xfffffffeu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float order_value(uint32_t k) {
-    return __uint_as_float((k & 0x80000000u) ? (k == 0xffffffffu ? 0x7fc00000u : k ^ 0x80000000u) : ~k);
+    return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); // (NaN's is a NaN)
 }
 __device__ __forceinline__ Order order_of(uint32_t bits, uint32_t id) { return (Order)bits << 32 | (0xffffffffu - id); }
 constexpr uint32_t INF_BITS = 0xff800000u, MINUS_INF_BITS = 0x007fffffu; // order_bits(+inf), order_bits(-inf)
@@ -159,7 +160,7 @@ struct Sums {
 // does not hold.
 template <typename T, int TH, typename Each>
 __device__ __noinline__ void take_one_by_one(Each each, int vocab, int n, Order *top, Order *best_of) {
-    Order last = ~0ull;
+    Order last = ~0ull; // above every token's
     auto next = [&]() { // this thread's largest below the last one taken
         Order o = 0;
         each([&](float f, long long id) {

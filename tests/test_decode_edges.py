@@ -60,3 +60,17 @@ def test_a_nan_anywhere_makes_its_row_nan_and_comes_first(rows, vocab, dt, gpu):
             assert np.array_equal(c[rest], g[rest])
         assert np.isnan(got[0][hit]).all() and np.isnan(got[1][hit]).all() and np.isnan(got[3][hit]).all(), (k, hit)
         assert np.array_equal(got[2][hit], order_with_nan(bad[hit])[:, :top]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [600, 5003, 300001])
+def test_rows_of_many_nans_give_the_lowest_ids(vocab, dt, gpu):
+    """Nothing but NaN, NaN from id 0 on and then values, and every other id: more of them than are collected before they are ranked."""
+    v = np.zeros((3, vocab), np.float32)
+    v[0], v[1, :580], v[2, ::2] = np.nan, np.nan, np.nan
+    v[1, 590] = 3.0
+    for rows in (v, np.tile(v, (100, 1))) if vocab < 300001 else (v,):
+        got = run_log_probs(rows, np.zeros(len(rows)), 32, gpu, dt)
+        assert np.isnan(got[0]).all() and np.isnan(got[1]).all() and np.isnan(got[3]).all()
+        assert np.array_equal(got[2], order_with_nan(rows)[:, :32])
