@@ -31,7 +31,7 @@ constexpr int LIST = 64;             // thread maxima that the bound is taken fr
 constexpr int MOST = 512;          // values collected
 constexpr int MAX_RANKS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float NO_REFERENCE = -1e38f, LOWEST = -1e38f; // values below LOWEST count as it: their t is finite and 2^t is 0
+constexpr float LOWEST = -1e38f; // values below it count as it: their t is finite and 2^t is 0
 using Order = unsigned long long;
 
 // larger value = larger word; -0 counts as +0, NaN as the largest; 0 is no value's word, nor is the largest one: a token's Order lies
@@ -58,10 +58,12 @@ __device__ __forceinline__ float exp2_approx(float t) {
 }
 
 // A chunk's values, and its largest (NaN if there is one): `wide` words hold the places' largest so far, 16-bit types two places a
-// word.  raised() is the chunk with values below LOWEST (and NaN) lifted to about that.
+// word.  raised() is the chunk with values below LOWEST (and NaN) lifted to about that, or to the type's lowest; START is the reference
+// before any value: so far above those that their powers are 0 from the first one on.
 template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     static constexpr int N = 4;
+    static constexpr float START = -1e38f;
     static constexpr uint32_t MINUS_INF = 0xff800000u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
@@ -72,6 +74,7 @@ template <> struct Chunk<float> {
 };
 template <> struct Chunk<__half> {
     static constexpr int N = 8;
+    static constexpr float START = -94300.f; // the lowest's t: -204 (from -1e38 it was +inf, and every masked row went the long way below)
     static constexpr uint32_t MINUS_INF = 0xfc00fc00u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -95,6 +98,7 @@ template <> struct Chunk<__half> {
 };
 template <> struct Chunk<__nv_bfloat16> {
     static constexpr int N = 8;
+    static constexpr float START = -1e38f;
     static constexpr uint32_t MINUS_INF = 0xff80ff80u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -238,7 +242,7 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
         return r;
     };
     // the largest values of the thread's best and second-best group of chunks (NaN above all), and where the best one begins
-    float c = NO_REFERENCE, best = -INFINITY, second = -INFINITY;
+    float c = Chunk<T>::START, best = -INFINITY, second = -INFINITY;
     int best_at = 0;
     unsigned long long s2 = 0, w2 = 0; // pairs of sums
     const unsigned long long log2e2 = pack2f(LOG2E, LOG2E);
@@ -448,7 +452,7 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
         if (tid == 0) meet[0] = c, meet[1] = s, meet[2] = w, slice_bits = bits;
         cluster_sync();
         if (rank == 0) {
-            float cs = NO_REFERENCE;
+            float cs = Chunk<T>::START;
             bits = 0;
             for (int r = 0; r < ranks; r++) cs = fmaxf(cs, load_peer(&meet[0], r)), bits = max(bits, load_peer(&slice_bits, r));
             s = w = 0.f;
@@ -478,7 +482,7 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
     if (tid == 0) redo = !nothing && !broken && !(s > 0.f), slice_bits = bits;
     __syncthreads();
     if (redo) {
-        // values whose t overflows: the lowest of f32 or bf16 and nothing above.  Differences to the largest are exact enough.
+        // values whose powers are all 0: about the type's lowest and nothing above.  Differences to the largest are exact enough.
         const float m = order_value(slice_bits);
         s = w = 0.f;
         for (int j = tid; j < vocab; j += TH) {

@@ -74,3 +74,55 @@ def test_rows_of_many_nans_give_the_lowest_ids(vocab, dt, gpu):
         got = run_log_probs(rows, np.zeros(len(rows)), 32, gpu, dt)
         assert np.isnan(got[0]).all() and np.isnan(got[1]).all() and np.isnan(got[3]).all()
         assert np.array_equal(got[2], order_with_nan(rows)[:, :32])
+
+
+# ------------------------------------------------------------------------------------------------ masks and values far from zero
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 9, 1003, 20001])
+def test_minus_infinity_is_not_the_type_s_lowest_value(vocab, dt, gpu):
+    """Rows whose largest value is the type's lowest or next to it, with and without -inf beside it; odd rows lie off the 16-byte
+    boundary, so that their partial chunks are filled up."""
+    low = np.float32(LOWEST[dt])
+    near = round_to(dt, np.array([low * (1 - k * HALF[dt]) for k in range(1, 9)], np.float32))  # 1 .. 8 half steps or so above
+    rng = np.random.default_rng(82)
+    v = np.full((16, vocab), low, np.float32)
+    v[1] = -np.inf
+    v[1, vocab // 2] = low
+    v[2, rng.random(vocab) < 0.5] = -np.inf
+    v[2, vocab - 1] = low
+    v[3] = -np.inf
+    v[4, 0] = near[7]
+    for r in range(5, 13):
+        v[r] = np.where(rng.random(vocab) < 0.7, -np.inf, low)
+        v[r, rng.integers(vocab)] = near[r - 5]
+    v[13], v[14, 0], v[15] = near[3], -np.inf, near[rng.integers(0, 8, vocab)]
+    for tokens in (np.zeros(16, int), v.argmax(1)):
+        lp_check(v, tokens, min(vocab, 5), gpu, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(1, 51865), (12, 51865), (320, 12001), (1, 300001)])
+def test_rows_masked_in_stretches(rows, vocab, dt, gpu):
+    """-inf over a prefix, a suffix, all but a few in the middle, and at random: threads that see nothing else first, or at all."""
+    rng = np.random.default_rng(83)
+    v = round_to(dt, 3 * rng.standard_normal((rows, vocab), dtype=np.float32))
+    for k in range(0, 6, rows if rows < 6 else 6):
+        m = v.copy()
+        for r in range(rows):
+            how = (k + r) % 6
+            if how == 0:
+                m[r, :vocab * 9 // 10] = -np.inf
+            elif how == 1:
+                m[r, 40000 % vocab:] = -np.inf
+            elif how == 2:
+                m[r, :vocab // 2], m[r, vocab // 2 + 50:] = -np.inf, -np.inf
+            elif how == 3:
+                m[r, rng.random(vocab) < 0.9] = -np.inf
+            elif how == 4:
+                m[r, :vocab - 1] = -np.inf
+            else:
+                m[r, rng.random(vocab) < 0.33] = -np.inf
+        lp_check(m, m.argmax(1), 32, gpu, dt)
