@@ -10,7 +10,9 @@
 //    those threads read their chunks again (from L2) and collect what reaches it, a few more values than asked for.  Each counts
 //    how many are larger, which is its place.  Rows with more ties than the collection holds take the values one by one.
 //  * What is not finite: -inf counts as the type's lowest or -1e38, a power of zero.  A row that has a NaN or +inf is known by its
-//    largest value.  A row of nothing but -inf, or of values below -1e38 (f32's and bf16's lowest as a mask), has S = 0.
+//    largest value, a row of nothing but -inf too.
+//  * c is rounded as v log2(e) is not.  Rows so far from zero that this shows, and rows that never reach the first reference (f32's and
+//    bf16's lowest as a mask), take the differences v - max first, in a second pass.
 //
 // 2048 bf16 rows of 51865, 20 likeliest: 53 us, 4.0 TB/s; without the likeliest 40, 5.3 TB/s: 9.4 instructions a value at 2.9 a cycle
 // and SM, of them one exponential at 16 a cycle.  One f16 row 7.1 us: 4000 of 12000 cycles are the pass of one SM, the rest steps that
@@ -479,10 +481,13 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
     // ---- the row, in the first warp, which has c, s, w and the largest value's bits
     bool nothing = bits <= MINUS_INF_BITS;
     const bool broken = bits >= INF_BITS; // +inf or NaN
-    if (tid == 0) redo = !nothing && !broken && !(s > 0.f), slice_bits = bits;
+    // The reference serves where the largest value's power is an ordinary number: it lies 8 powers below the largest at most, and where it
+    // does not, it was rounded (beyond 2^24) or is none of the row's.  Then, or where a t overflowed, the sums are taken again.
+    if (tid == 0) redo = !nothing && !broken && !(fabsf(fmaf(order_value(bits), LOG2E, -c)) <= 9.f && w == w), slice_bits = bits;
     __syncthreads();
     if (redo) {
-        // values whose powers are all 0: about the type's lowest and nothing above.  Differences to the largest are exact enough.
+        // rows of the type's lowest and nothing above, of a finite mask over everything, of logits beyond 1e7: differences to the largest
+        // are exact enough
         const float m = order_value(slice_bits);
         s = w = 0.f;
         for (int j = tid; j < vocab; j += TH) {

@@ -126,3 +126,27 @@ def test_rows_masked_in_stretches(rows, vocab, dt, gpu):
             else:
                 m[r, rng.random(vocab) < 0.33] = -np.inf
         lp_check(m, m.argmax(1), 32, gpu, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("vocab", [8, 1003, 51865])
+def test_logits_far_from_zero(vocab, dt, gpu):
+    """Rows of one value of any size and sign (a finite mask over everything), alone or with a smaller one in between, and rows that
+    span most of the type's range: log probabilities follow the differences, which are exact."""
+    rng = np.random.default_rng(84)
+    top = 4 if dt == F16 else 38
+    sizes = (10.0 ** rng.uniform(3, top, 40)).astype(np.float32)
+    sizes = sizes[sizes < -LOWEST[dt]]
+    sizes = round_to(dt, np.concatenate([sizes, [1e4, 3e4] if dt == F16 else [1e9, 2e9, 1e10, 3e10, 1e12, 1e30, 1.4e38, 1.9e38, 2.3e38, 2.4e38, 3.3e38]]).astype(np.float32))
+    n = len(sizes)
+    v = np.concatenate([np.repeat(s * sizes[:, None], vocab, 1) for s in (1, -1)])
+    v[:n:2, vocab // 3] = v[:n:2, 0] / 2
+    v[n::2, vocab // 3] = np.maximum(v[n::2, 0] * np.float32(1.5), LOWEST[dt] / 1.25)
+    v[n::2, vocab // 3] = np.minimum(v[n::2, vocab // 3], v[n::2, 0])
+    v[n + 1::4, 0] = LOWEST[dt]
+    v[3::4, -1] = -np.inf
+    v = round_to(dt, v)
+    assert np.isfinite(v).any(1).all()
+    lp_check(v, v.argmax(1), 5, gpu, dt)
+    lp_check(v, np.zeros(len(v), int), 0, gpu, dt)
