@@ -371,11 +371,11 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
         if (tid < p.top) top[tid] = 0;
         __syncthreads();
         const uint32_t least = max(bound, 1u);
-        auto push = [&](float f, int id) {
+        auto push = [&](float f, uint32_t id) { // (an id before the row's first or behind its last is no less than vocab)
             const uint32_t b = order_bits(f);
-            if (b >= least && (unsigned)id < (unsigned)vocab) {
+            if (b >= least && id < (uint32_t)vocab) {
                 const int to = atomicAdd(&count, 1);
-                if (to < MOST) found[to] = order_of(b, (uint32_t)id);
+                if (to < MOST) found[to] = order_of(b, id);
             }
         };
         // A thread that has some of the largest looks at its best group again; where the second-best has some too, it is marked, and
@@ -392,14 +392,14 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
                     float f[N];
                     Chunk<T>::values(r, f);
 #pragma unroll
-                    for (int k = 0; k < N; k++) push(f[k], at * N - shift + k);
+                    for (int k = 0; k < N; k++) push(f[k], (uint32_t)at * N - shift + k);
                 }
             }
             if (odd >= 0) {
                 float f[N];
                 Chunk<T>::values(guarded(odd), f);
 #pragma unroll
-                for (int k = 0; k < N; k++) push(f[k], odd * N - shift + k);
+                for (int k = 0; k < N; k++) push(f[k], (uint32_t)odd * N - shift + k);
             }
         }
         __syncthreads();
@@ -422,7 +422,7 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
                     float mine_of_it = f[0];
 #pragma unroll
                     for (int k = 1; k < N; k++) mine_of_it = lane == k ? f[k] : mine_of_it;
-                    if (lane < N) push(mine_of_it, (at0 + src * TH) * N - shift + lane);
+                    if (lane < N) push(mine_of_it, (uint32_t)(at0 + src * TH) * N - shift + lane);
                 }
             }
         __syncthreads();
@@ -490,7 +490,7 @@ template <typename T, int TH> __global__ void __launch_bounds__(TH, TH == 256 ? 
         // are exact enough
         const float m = order_value(slice_bits);
         s = w = 0.f;
-        for (int j = tid; j < vocab; j += TH) {
+        for (uint32_t j = tid; j < (uint32_t)vocab; j += TH) { // (vocab + TH may pass 2^31)
             const float t = fmaxf((to_f32(v[j]) - m) * LOG2E, LOWEST), e = exp2_approx(t);
             s += e;
             w = fmaf(e, t, w);

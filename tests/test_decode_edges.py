@@ -150,3 +150,32 @@ def test_logits_far_from_zero(vocab, dt, gpu):
     assert np.isfinite(v).any(1).all()
     lp_check(v, v.argmax(1), 5, gpu, dt)
     lp_check(v, np.zeros(len(v), int), 0, gpu, dt)
+
+
+# ------------------------------------------------------------------------------------------------ long rows
+
+@pytest.mark.gpu
+def test_the_longest_row_that_is_taken(gpu):
+    """2^31 - 1 logits of the type's lowest value, whose differences are taken in a second pass, and two at the end that are larger."""
+    import torch
+    vocab, lib = 2**31 - 1, _lib.load()
+    v = torch.full((vocab,), LOWEST[BF16], dtype=torch.bfloat16, device="cuda")
+    ent, given, tops, ids = (torch.zeros(n, dtype=t, device="cuda") for n, t in ((1, torch.float32), (1, torch.float32), (2, torch.float32), (2, torch.int32)))
+    tokens = torch.tensor([vocab - 1], dtype=torch.int32, device="cuda")
+    p = _lib.rt_log_probs()
+    p.dt, p.top, p.rows, p.vocab, p.ld, p.logits, p.tokens = _lib.RT_BF16, 2, 1, vocab, vocab, v.data_ptr(), tokens.data_ptr()
+    p.log_prob, p.entropy, p.top_ids, p.top_log_prob = given.data_ptr(), ent.data_ptr(), ids.data_ptr(), tops.data_ptr()
+
+    def run():
+        torch.cuda.synchronize()
+        _lib.check(lib.rt_log_probs_launch(gpu._h, ctypes.byref(p), None))
+        gpu.sync()
+        return given.item(), ent.item(), ids.tolist(), tops.tolist()
+
+    # every power is 1, so the sums are exact but for the last ones: a few steps of their 2^31, and of log2's 31 and ln 2
+    slack = (16 + 8 * 21.5) * E24
+    one, h, first, tp = run()
+    assert abs(one + np.log(vocab)) <= slack and abs(h - np.log(vocab)) <= slack and first == [0, 1] and np.abs(np.array(tp) + np.log(vocab)).max() <= slack
+    v[-1] = v[-3] = -3.2e38
+    one, h, first, tp = run()
+    assert abs(one + np.log(2)) <= slack and abs(h - np.log(2)) <= slack and first == [vocab - 3, vocab - 1] and np.abs(np.array(tp) + np.log(2)).max() <= slack
