@@ -179,3 +179,39 @@ def test_the_longest_row_that_is_taken(gpu):
     v[-1] = v[-3] = -3.2e38
     one, h, first, tp = run()
     assert abs(one + np.log(2)) <= slack and abs(h - np.log(2)) <= slack and first == [vocab - 3, vocab - 1] and np.abs(np.array(tp) + np.log(2)).max() <= slack
+
+
+#: of an f32 sum, relative to the sum of the terms: a thread adds 2048 terms at most before its sum joins the others, each addition off
+#: by half a step; an exponential by two steps of 2^-23 and its exponent's rounding; the sums' sum and the trees by as much as 300 more
+LONG = (2048 + 300 + 16) * E24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,vocab,rows", [(F32, 2**27 + 3, 1), (F16, 2**28 + 5, 1), (BF16, 2**28, 2), (F16, 2**22 + 1, 300), (F16, 2**31 - 1, 1), (BF16, 2**31 - 9, 1)])
+def test_rows_of_many_millions(dt, vocab, rows, gpu):
+    """A thread's first values are larger than all that follow, which are equal: its sums take the same term over and over, whose
+    roundings all fall to the same side.  The last two ids are the likeliest, then the first two."""
+    import torch
+    kind = {F32: torch.float32, F16: torch.half, BF16: torch.bfloat16}[dt]
+    v = torch.full((rows, vocab), 1.0, dtype=kind, device="cuda")
+    for k in range(8):
+        v[:, max(0, vocab // 8 * k - 64):vocab // 8 * k + 16500] = 4.3125
+    v[:, -2:] = 5.0
+    ent, ids, tops, given = (torch.zeros(rows, n, dtype=t, device="cuda") for n, t in ((1, torch.float32), (4, torch.int32), (4, torch.float32), (1, torch.float32)))
+    tokens = torch.full((rows,), vocab - 1, dtype=torch.int32, device="cuda")
+    p = _lib.rt_log_probs()
+    p.dt, p.top, p.rows, p.vocab, p.ld, p.logits, p.tokens = int(dt), 4, rows, vocab, vocab, v.data_ptr(), tokens.data_ptr()
+    p.log_prob, p.entropy, p.top_ids, p.top_log_prob = given.data_ptr(), ent.data_ptr(), ids.data_ptr(), tops.data_ptr()
+    torch.cuda.synchronize()
+    _lib.check(_lib.load().rt_log_probs_launch(gpu._h, ctypes.byref(p), None))
+    gpu.sync()
+    kinds = np.array([5.0, 4.3125, 1.0])
+    ahead = int((v[0] == 4.3125).sum())
+    weights = np.array([2, ahead, vocab - 2 - ahead]) * np.exp(kinds)
+    logp = kinds - np.log(weights.sum())
+    assert np.array_equal(ids.cpu().numpy(), np.tile([vocab - 2, vocab - 1, 0, 1], (rows, 1)))
+    slack = LONG + 4 * E24 * 25  # (log2 and the last sums are f32 numbers of at most 25)
+    assert np.abs(tops.double().cpu().numpy() - logp[[0, 0, 1, 1]]).max() <= slack
+    assert np.abs(given.double().cpu().numpy() - logp[0]).max() <= slack
+    # entropy = ln S - sum e t / S: both lose LONG, the second times its terms' size, 5.8 powers of two at most
+    assert np.abs(ent.double().cpu().numpy() + (weights * logp).sum() / weights.sum()).max() <= slack + 2 * 5.8 * LONG
