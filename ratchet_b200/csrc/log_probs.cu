@@ -299,27 +299,32 @@ template <typename T, int TH, bool LONG> __global__ void __launch_bounds__(TH, T
         return sum;
     };
     int left = my_chunks, part = 0;
-    while (left >= GROUP) {
-        for (const int stop = LONG ? max(left - SEGMENT * GROUP, GROUP - 1) : GROUP - 1; left > stop; left -= GROUP, part = (part + 1) % GROUPS) {
-            copy_wait<GROUPS - 1>();
-            uint4 r[GROUP];
+    auto step = [&]() {
+        copy_wait<GROUPS - 1>();
+        uint4 r[GROUP];
 #pragma unroll
-            for (int k = 0; k < GROUP; k++) r[k] = place[(part * GROUP + k) * TH];
-            uint32_t wide = wide_of<T>(r[0]);
+        for (int k = 0; k < GROUP; k++) r[k] = place[(part * GROUP + k) * TH];
+        uint32_t wide = wide_of<T>(r[0]);
 #pragma unroll
-            for (int k = 1; k < GROUP; k++) wide = Chunk<T>::wider(wide, wide_of<T>(r[k]));
-            const float m = Chunk<T>::widest(wide);
-            raise(m);
-            rank_group(m, my_chunks - left);
-            ask(part); // (into the places just read)
+        for (int k = 1; k < GROUP; k++) wide = Chunk<T>::wider(wide, wide_of<T>(r[k]));
+        const float m = Chunk<T>::widest(wide);
+        raise(m);
+        rank_group(m, my_chunks - left);
+        ask(part); // (into the places just read)
 #pragma unroll
-            for (int k = 0; k < GROUP; k++) add(r[k]);
-        }
-        if (LONG && left >= GROUP) {
+        for (int k = 0; k < GROUP; k++) add(r[k]);
+        left -= GROUP, part = (part + 1) % GROUPS;
+    };
+    if constexpr (LONG) {
+        while (left >= GROUP) {
+            for (const int stop = max(left - SEGMENT * GROUP, GROUP - 1); left > stop;) step();
+            if (left < GROUP) break;
             const Sums sum = left + SEGMENT * GROUP < my_chunks ? with_kept() : Sums{c, sum2(s2), sum2(w2)};
             kept[0][tid] = sum.c, kept[1][tid] = sum.s, kept[2][tid] = sum.w;
             s2 = w2 = 0;
         }
+    } else {
+        while (left >= GROUP) step();
     }
     copy_wait<0>();
     for (int k = 0; k < left; k++) {
@@ -508,7 +513,7 @@ template <typename T, int TH, bool LONG> __global__ void __launch_bounds__(TH, T
         for (uint32_t j = tid; j < (uint32_t)vocab;) { // (vocab + TH may pass 2^31)
             float ps = 0.f, pw = 0.f;
             const uint32_t stop = min((uint32_t)vocab, j + 8 * SEGMENT * TH);
-#pragma unroll 8
+#pragma unroll 4
             for (; j < stop; j += TH) {
                 const float t = fmaxf((to_f32(v[j]) - m) * LOG2E, LOWEST), e = exp2_approx(t);
                 ps += e;

@@ -142,7 +142,7 @@ def test_logits_far_from_zero(vocab, dt, gpu):
     n = len(sizes)
     v = np.concatenate([np.repeat(s * sizes[:, None], vocab, 1) for s in (1, -1)])
     v[:n:2, vocab // 3] = v[:n:2, 0] / 2
-    v[n::2, vocab // 3] = np.maximum(v[n::2, 0] * np.float32(1.5), LOWEST[dt] / 1.25)
+    v[n::2, vocab // 3] = np.maximum(v[n::2, 0].astype(np.float64) * 1.5, LOWEST[dt] / 1.25)
     v[n::2, vocab // 3] = np.minimum(v[n::2, vocab // 3], v[n::2, 0])
     v[n + 1::4, 0] = LOWEST[dt]
     v[3::4, -1] = -np.inf
