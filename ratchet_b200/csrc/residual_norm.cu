@@ -13,6 +13,7 @@
 // 20 warps, and the start.  Rows of 2561, all off the 16-byte boundary, with a sixth warp for one value: 53 us.  One row: 3.4 us, the
 // launch.
 #include <algorithm>
+#include <cfloat>
 #include <utility>
 
 #include "common.cuh"
@@ -320,17 +321,19 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 // takes such rows only, and its threads' values sit at the same places in each: s values before those of an aligned row.  The
 // 16-byte words that hold the row are copied, which in the first and the last row would reach outside the tensor: those are read where
 // they are.  VEC = 1: the same copies for operands that differ in s, value by value.
-// PLAIN: no means and no biases, which leaves the registers for more teams.
+// Form: PLAIN has no means and no biases, which leaves the registers for more teams; GATED a gate behind a bias, where an infinite gate
+// may not be folded into both (8192 bf16 rows of 2560, layer norms, a gate a sequence: 46.8 us, 45.3 without that).
+enum Form { PLAIN, MEANS, GATED };
 constexpr int N = 16, MAX_STAGES = 4, MAX_TEAMS = 8, WALK_SMEM = 200 * 1024;
 constexpr int MIN_WALK_D = 8; // 16 bytes: the words of a row that is neither first nor last lie in the tensor
-template <bool PLAIN> constexpr int WALK_THREADS = PLAIN ? 640 : 512; // of an SM, at 96 or 128 registers
+template <Form F> constexpr int WALK_THREADS = F == PLAIN ? 640 : 512; // of an SM, at 96 or 128 registers
 
 template <bool ALIGNED> __host__ __device__ constexpr int walk_operand_bytes(int row_bytes) { // of a stage
     return ALIGNED ? row_bytes : (row_bytes + 15) / 16 * 16 + 16;
 }
 
-template <typename T, int VEC, bool WARP, bool PLAIN, bool SHIFT>
-__global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, WARP ? 2 : 1) residual_norm_walk_kernel(const __grid_constant__ ResidualNormParams p, int share, int stages, int period) {
+template <typename T, int VEC, bool WARP, Form F, bool SHIFT>
+__global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<F>, WARP ? 2 : 1) residual_norm_walk_kernel(const __grid_constant__ ResidualNormParams p, int share, int stages, int period) {
     constexpr int C = N / VEC;
     constexpr bool ALIGNED = VEC > 1 && !SHIFT;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -411,13 +414,15 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
     };
     if (p.pre.weight) take_param(p.pre.weight, p.pre.f32, wx);
     else fill(wx, 1.f);
-    if (!PLAIN && p.pre.bias) take_param(p.pre.bias, p.pre.f32, bx);
+    if (F != PLAIN && p.pre.bias) take_param(p.pre.bias, p.pre.f32, bx);
     else fill(bx, 0.f);
+    bool wild = false; // an infinite b g before a bias: the thread's values go by the formula's own order
     auto take_gate = [&](long long which) {
         float w[N];
+        wild = false;
         if (p.post.weight) take_param(p.post.weight, p.post.f32, w);
         else fill(w, 1.f);
-        if (!PLAIN && p.post.bias) take_param(p.post.bias, p.post.f32, add);
+        if (F != PLAIN && p.post.bias) take_param(p.post.bias, p.post.f32, add);
         else fill(add, 0.f);
         if (p.gate) take_param((const T *)p.gate + which * d, sizeof(T) == 4, mul);
         else fill(mul, 1.f);
@@ -425,6 +430,8 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
         for (int j = 0; j < N; j++) { // (past the row's end h stays 0)
             const float m = valid(j) ? p.b * mul[j] : 0.f;
             mul[j] = valid(j) ? m * w[j] : 0.f;
+            if (F == PLAIN || !p.post.bias) continue; // (add is 0, whatever m is)
+            if (F == GATED && !(fabsf(m) <= FLT_MAX)) wild = true;
             add[j] = valid(j) ? m * add[j] : 0.f;
         }
     };
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
             const unsigned long long sc = pack2f(scale, scale);
 #pragma unroll
             for (int j = 0; j < N; j += 2)
-                if (PLAIN) unpack2f(mul2(mul2(pack2f(u[j], u[j + 1]), sc), pack2f(m[j], m[j + 1])), u[j], u[j + 1]);
+                if (F == PLAIN) unpack2f(mul2(mul2(pack2f(u[j], u[j + 1]), sc), pack2f(m[j], m[j + 1])), u[j], u[j + 1]);
                 else unpack2f(fma2(mul2(pack2f(u[j], u[j + 1]), sc), pack2f(m[j], m[j + 1]), pack2f(b[j], b[j + 1])), u[j], u[j + 1]);
         };
         auto store = [&](T *to) {
@@ -525,8 +532,23 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
 #pragma unroll
                 for (int j = 0; j < VEC; j++) u[c * VEC + j] = v[j];
             }
-            if (!PLAIN && p.post.kind == RT_NORM_LAYER) centre(total(false, 0));
-            scaled(p.post.kind != RT_NORM_NONE ? rsqrtf(total(true, 1) + p.post.eps) : 1.f, mul, add);
+            if (F != PLAIN && p.post.kind == RT_NORM_LAYER) centre(total(false, 0));
+            const float scale = p.post.kind != RT_NORM_NONE ? rsqrtf(total(true, 1) + p.post.eps) : 1.f;
+            if (F == GATED && wild) {
+                const long long which = p.rows_per_gate ? row_of(i) / p.rows_per_gate : 0;
+                auto param = [&](const void *of, int f32, int at) { return f32 ? ((const float *)of)[at] : to_f32(((const T *)of)[at]); };
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    if (!valid(j)) continue; // (0)
+                    const int at = index(j);
+                    u[j] *= scale;
+                    if (p.post.weight) u[j] *= param(p.post.weight, p.post.f32, at);
+                    u[j] = (u[j] + param(p.post.bias, p.post.f32, at)) * p.b;
+                    if (p.gate) u[j] *= to_f32(((const T *)p.gate)[which * d + at]);
+                }
+            } else {
+                scaled(scale, mul, add);
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < N; j++) u[j] = -0.f; // (a r - 0 is a r)
@@ -545,7 +567,7 @@ __global__ void __launch_bounds__(WARP ? 32 * MAX_TEAMS : WALK_THREADS<PLAIN>, W
         }
         if (p.h) store(hp);
         if (p.pre.kind != RT_NORM_NONE) {
-            if (!PLAIN && p.pre.kind == RT_NORM_LAYER) centre(total(false, 2));
+            if (F != PLAIN && p.pre.kind == RT_NORM_LAYER) centre(total(false, 2));
             const float scale = rsqrtf(total(true, 3) + p.pre.eps);
             refill();
             scaled(scale, wx, bx);
@@ -673,11 +695,11 @@ template <typename T, int VEC> __global__ void __launch_bounds__(1024) residual_
     });
 }
 
-template <typename T, int VEC, bool WARP, bool PLAIN, bool SHIFT> cudaError_t launch_walk(const ResidualNormParams &p, int period, int sm_count, cudaStream_t stream) {
-    const auto kernel = residual_norm_walk_kernel<T, VEC, WARP, PLAIN, SHIFT>;
+template <typename T, int VEC, bool WARP, Form F, bool SHIFT> cudaError_t launch_walk(const ResidualNormParams &p, int period, int sm_count, cudaStream_t stream) {
+    const auto kernel = residual_norm_walk_kernel<T, VEC, WARP, F, SHIFT>;
     const int threads = WARP ? 32 : (p.d + (SHIFT ? VEC - 1 : 0) + N * 32 - 1) / (N * 32) * 32, teams = WARP ? MAX_TEAMS : 1;
     const int stage = teams * walk_operand_bytes<(VEC > 1 && !SHIFT)>(p.d * (int)sizeof(T)) * ((p.r != nullptr) + (p.y != nullptr));
-    const int per_sm = WALK_THREADS<PLAIN> / (threads * teams);
+    const int per_sm = WALK_THREADS<F> / (threads * teams);
     const int stages = std::max(2, std::min(MAX_STAGES, WALK_SMEM / per_sm / stage));
     static SmemAttr attr;
     cudaError_t e = attr.ensure(kernel, (size_t)WALK_SMEM);
@@ -688,10 +710,15 @@ template <typename T, int VEC, bool WARP, bool PLAIN, bool SHIFT> cudaError_t la
     return launch_pdl(kernel, dim3((unsigned)((used + teams - 1) / teams)), dim3(threads, teams), (size_t)stages * stage, stream, p, (int)share, stages, period);
 }
 
-template <typename T, int VEC, bool SHIFT> cudaError_t launch_walks(const ResidualNormParams &p, bool plain, int period, int sm_count, cudaStream_t stream) {
-    if (p.d + (SHIFT ? VEC - 1 : 0) <= 32 * N)
-        return plain ? launch_walk<T, VEC, true, true, SHIFT>(p, period, sm_count, stream) : launch_walk<T, VEC, true, false, SHIFT>(p, period, sm_count, stream);
-    return plain ? launch_walk<T, VEC, false, true, SHIFT>(p, period, sm_count, stream) : launch_walk<T, VEC, false, false, SHIFT>(p, period, sm_count, stream);
+template <typename T, int VEC, Form F, bool SHIFT> cudaError_t launch_form(const ResidualNormParams &p, int period, int sm_count, cudaStream_t stream) {
+    return p.d + (SHIFT ? VEC - 1 : 0) <= 32 * N ? launch_walk<T, VEC, true, F, SHIFT>(p, period, sm_count, stream)
+                                                 : launch_walk<T, VEC, false, F, SHIFT>(p, period, sm_count, stream);
+}
+
+template <typename T, int VEC, bool SHIFT> cudaError_t launch_walks(const ResidualNormParams &p, Form form, int period, int sm_count, cudaStream_t stream) {
+    return form == PLAIN   ? launch_form<T, VEC, PLAIN, SHIFT>(p, period, sm_count, stream)
+           : form == MEANS ? launch_form<T, VEC, MEANS, SHIFT>(p, period, sm_count, stream)
+                           : launch_form<T, VEC, GATED, SHIFT>(p, period, sm_count, stream);
 }
 
 template <typename T, int VEC, int C, bool EARLY> cudaError_t launch_row(const ResidualNormParams &p, cudaStream_t stream) {
@@ -708,12 +735,13 @@ template <typename T, int VEC> cudaError_t launch_t(const ResidualNormParams &p,
     const bool few = p.rows <= (long long)sm_count * (WAVE / threads) || (p.d <= 32 * N && p.rows <= 2 * MAX_TEAMS * sm_count);
     if (p.d <= 4096 && (few || p.d < MIN_WALK_D)) return launch_row<T, VEC, EARLY_C, true>(p, stream);
     const bool plain = p.post.kind != RT_NORM_LAYER && p.pre.kind != RT_NORM_LAYER && !p.post.bias && !p.pre.bias;
-    const int longest = (plain ? WALK_THREADS<true> : WALK_THREADS<false>) * N;
+    const Form form = plain ? PLAIN : p.post.bias && (p.gate || !(fabsf(p.b) <= FLT_MAX)) ? GATED : MEANS;
+    const int longest = (plain ? WALK_THREADS<PLAIN> : WALK_THREADS<MEANS>) * N;
     // operands that lie alike go by 16-byte words (8192 bf16 rows of 2561: 53 us, 71 value by value; 52000 rows of 383: 67 and 67, with
     // means and biases 93 and 102)
     if constexpr (VEC == 1)
-        if (period && p.d + WORD - 1 <= longest) return launch_walks<T, WORD, true>(p, plain, period, sm_count, stream);
-    if (p.d <= longest) return launch_walks<T, VEC, false>(p, plain, 1, sm_count, stream);
+        if (period && p.d + WORD - 1 <= longest) return launch_walks<T, WORD, true>(p, form, period, sm_count, stream);
+    if (p.d <= longest) return launch_walks<T, VEC, false>(p, form, 1, sm_count, stream);
     // longer rows, 32 values a thread in registers while 512 threads hold them (2048 bf16 rows of 10240: 51 us, 103 with the loops;
     // value by value, rows of 9001, 282 and 128)
     if constexpr (VEC > 1)

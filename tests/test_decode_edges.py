@@ -215,3 +215,39 @@ def test_rows_of_many_millions(dt, vocab, rows, gpu):
     assert np.abs(given.double().cpu().numpy() - logp[0]).max() <= slack
     # entropy = ln S - sum e t / S: both lose LONG, the second times its terms' size, 5.8 powers of two at most
     assert np.abs(ent.double().cpu().numpy() + (weights * logp).sum() / weights.sum()).max() <= slack + 2 * 5.8 * LONG
+
+
+# ------------------------------------------------------------------------------------------------ norms
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("post", [None, "rms", "layer", "layer+bias"])
+@pytest.mark.parametrize("d", [40, 520, 1003, 2560])
+def test_infinite_gates_do_the_same_to_few_rows_and_to_many(d, post, dt, gpu):
+    """h = a r + b g post(block) where g is infinite: +-inf by the block's sign at that place, NaN where the block is 0; the rest as ever."""
+    rng, rows = np.random.default_rng(91), 5003
+    r, y = (round_to(dt, rng.standard_normal((rows, d), dtype=np.float32)) for _ in range(2))
+    if post is None:
+        y[7, 3] = 0.0
+    w, b = round_to(dt, rng.uniform(0.5, 2.0, d).astype(np.float32)), round_to(dt, rng.uniform(-2.0, 2.0, d).astype(np.float32))
+    gate = round_to(dt, rng.uniform(0.5, 1.5, d).astype(np.float32))
+    gate[[3, 17, d - 1]] = np.inf, -np.inf, np.inf
+    t = lambda a: Tensor.from_data(a, gpu, dt)  # noqa: E731
+    block = {None: None, "rms": lambda: RMSNorm(t(w)), "layer": lambda: LayerNorm(t(w)), "layer+bias": lambda: LayerNorm(t(w), t(b))}[post]
+    kind, bias = None if post is None else post.split("+")[0], b.astype(np.float64) if post == "layer+bias" else 0.0
+    truth = (kind, w.astype(np.float64), bias, np.float64(np.float32(1e-5)))
+    finite = np.isfinite(gate)
+    with np.errstate(invalid="ignore"):
+        (v, e), _ = norm_truth(r.astype(np.float64), y.astype(np.float64), np.where(finite, gate, 1.0).astype(np.float64), truth, (None, 1, 0, 0), 0.5, -2.0)
+        u, eu = norm_truth(None, y.astype(np.float64), None, truth, (None, 1, 0, 0), 1.0, -2.0)[0]
+        want = np.where(finite, v, gate.astype(np.float64) * u)
+    sure = finite | (np.abs(u) > 2 * eu) | (u == 0)  # (whose sign f32 has)
+    assert sure.mean() > 0.99
+    for pre in (None, LayerNorm(t(w))):
+        for n in (3, 100, rows):
+            mod = ResidualNorm(pre, block() if block else None, 0.5, -2.0)
+            h, x = mod.schedule(t(r[:n]), t(y[:n]), t(gate))
+            got = h.resolve().to(Device.CPU).to_f32().astype(np.float64)
+            same = (got == want[:n]) | (np.isnan(got) & np.isnan(want[:n])) | (finite & close(got, (want[:n], e[:n]), dt))
+            assert np.all(same | ~sure[:n]), (n, pre, np.argwhere(~(same | ~sure[:n]))[:4])
+            assert x is None or np.isnan(x.resolve().to(Device.CPU).to_f32()).all()
