@@ -1124,6 +1124,12 @@ rt_status rt_graph_resolve(rt_device *dev, const uint64_t *nodes, int32_t n, uin
 
 } // extern "C"
 
+// Every kernel reads and writes whole elements, f16 or f32 scales among them: an address off their boundary would fault on the device.
+static bool misaligned(const void *p, rt_dtype dt) {
+    const size_t size = !is_quantized(dt) ? dtype_size(dt) : dt == RT_Q8_0F ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(p) % size != 0;
+}
+
 // One node's launches.  `ov` names scratch areas that take the place of the plan's own (an executable's arena).
 static rt_status launch_node(rt_plan *plan, const void *lhs, const void *rhs, const void *bias, void *out, void *stream,
                              const rt_launch_opts *opts, const ScratchSet *ov) {
@@ -1150,6 +1156,9 @@ static rt_status launch_node(rt_plan *plan, const void *lhs, const void *rhs, co
         return fail(RT_ERR_ARG, "rt_matmul_launch: null operand");
     if (user_out == lhs || user_out == rhs || (s.has_bias && user_out == bias))
         return fail(RT_ERR_INVARIANT, "Matmul is never in place: out aliases an operand");
+    if (misaligned(lhs, s.desc.lhs_dt) || misaligned(rhs, s.desc.rhs_dt) || misaligned(user_out, s.out_dt) ||
+        (s.has_bias && misaligned(bias, s.desc.bias_dt)))
+        return fail(RT_ERR_ARG, "rt_matmul_launch: an operand is not aligned to its elements");
     CUDA_TRY(cudaSetDevice(plan->dev->ordinal));
     cudaStream_t st = stream ? (cudaStream_t)stream : plan->dev->stream;
     MatmulParams p = bound_params(plan, lhs, rhs, bias, out);
@@ -1662,6 +1671,8 @@ const char *rt_executable_kernel(const rt_executable *exe) { return exe ? exe->h
 rt_status rt_dequantize_device(rt_device *dev, rt_dtype dt, uint64_t numel, const void *src, void *dst, void *stream) {
     if (!dev || !src || !dst) return fail(RT_ERR_ARG, "rt_dequantize_device: null argument");
     if (!dtype_valid(dt) || !is_quantized(dt)) return fail(RT_ERR_DTYPE, "rt_dequantize_device: not a block format");
+    if (misaligned(src, dt) || misaligned(dst, dt == RT_Q8_0H ? RT_F16 : RT_F32))
+        return fail(RT_ERR_ARG, "rt_dequantize_device: an operand is not aligned to its elements");
     rt_segment seg[RT_MAX_SEGMENTS];
     int n = 0;
     Status st = dtype_segments(dt, numel, seg, &n);
