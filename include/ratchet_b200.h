@@ -62,8 +62,9 @@ typedef enum rt_dtype {
     RT_Q4_K = 7,  /* raw GGUF Q4_K super-blocks, 144 bytes per 256 values */
     /* 4-bit codes with an f16 scale and a zero point per group of 32, 64 or 128 consecutive values of a row (an
      * extension: the reference has no such format): value = (q - z) * s, exact in f32.  Operand of f16 and bf16
-     * activations.  Where the activations are many (a tensor-core GEMM) the values are rounded to f16 once, so
-     * |value| <= 65504 is the weight's part. */
+     * activations.  Up to 16 vectors the sums of q x and of z x are taken apart in f32: before its own rounding an
+     * output is off by (K / 64 + 174) 2^-24 of sum s (q + z) |x| at most.  Where the activations are many (a
+     * tensor-core GEMM) the values are rounded to f16 once, so |value| <= 65504 is the weight's part. */
     RT_Q4_G32 = 8,
     RT_Q4_G64 = 9,
     RT_Q4_G128 = 10

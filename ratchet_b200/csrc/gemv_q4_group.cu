@@ -16,6 +16,9 @@
 //  * Activations are staged in shared memory in the order the MMAs take them, with their sums by group; so are scales and zero
 //    points, a word a group (read from global memory by the lanes that need them they would be more requests than the codes).
 //  * f32 sums of a group times s, added in f32 over steps, warps and CTAs of the cluster in a fixed order.
+//  * q x and z x are summed apart, so f32 roundings go with sum s (q + z) |x| and not with sum s |q - z| |x|: (K / 64 + 174) 2^-24 of it
+//    at most by the count of additions, 2^-25 where it was looked for (codes at and next to zero points of 8 .. 31).  Beside f16's own
+//    rounding that shows in outputs 2^14 times smaller than their terms; a group of codes equal to its zero point adds as much, not 0.
 //
 // One vector, 51200 rows of 2560: 15.2 us with groups of 128 (4.5 TB/s), 16.6 of 64, 18.2 of 32; 2560 x 2560 3.7, the launch and two
 // trips to memory; 16 vectors 23.5 / 29 / 46: the epilogue of a group (FMAs by vectors, in pairs) and the masking bound those.  A
