@@ -274,10 +274,11 @@ class Executable:
         self.launches = int(_lib.load().rt_executable_launches(self._h))
         self.kernel = _lib.load().rt_executable_kernel(self._h).decode()
 
-    @staticmethod
-    def _resolved(t: "Tensor") -> None:
+    def _resolved(self, t: "Tensor") -> None:
         if t.op is None or not isinstance(t.storage, GpuBuffer):
             raise RatchetError(_lib.RT_ERR_ARG, "RT_ERR_ARG", "Executable nodes must be resolved op outputs")
+        if t.storage.device is not self.device:
+            raise RatchetError(_lib.RT_ERR_ARG, "RT_ERR_ARG", f"Executable on {self.device}: a node is on {t.storage.device}")
 
     def _bind(self, d: "_lib.rt_dispatch", t: "Tensor") -> None:
         self._resolved(t)

@@ -4,7 +4,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from ratchet_b200 import Device, DType, LayerNorm, RatchetError, ResidualNorm, RMSNorm, Tensor
+from ratchet_b200 import Device, DeviceRequest, DType, Executable, GpuBuffer, LayerNorm, Linear, RatchetError, ResidualNorm, RMSNorm, Tensor
 from ratchet_b200 import _lib
 from test_decode_ops import E24, close, lp_check, lp_truth, norm_truth
 from util import round_to
@@ -251,3 +251,23 @@ def test_infinite_gates_do_the_same_to_few_rows_and_to_many(d, post, dt, gpu):
             same = (got == want[:n]) | (np.isnan(got) & np.isnan(want[:n])) | (finite & close(got, (want[:n], e[:n]), dt))
             assert np.all(same | ~sure[:n]), (n, pre, np.argwhere(~(same | ~sure[:n]))[:4])
             assert x is None or np.isnan(x.resolve().to(Device.CPU).to_f32()).all()
+
+
+# ------------------------------------------------------------------------------------------------ CPU: executables
+
+def test_an_executable_refuses_nodes_of_another_device():
+    """Their memory belongs to the other GPU: a Matmul node, an operator with several outputs, and one of each."""
+    here, there = (Device(DeviceRequest.GPU, k) for k in range(2))
+
+    def on(device, *outs):
+        for t in outs:
+            t.storage = GpuBuffer.__new__(GpuBuffer)
+            t.storage.device, t.storage._h, t.storage.ptr, t.storage.size = device, None, 1 << 20, 1 << 16
+        return list(outs)
+
+    t = lambda *shape: Tensor(shape, F16, there)  # noqa: E731
+    product = on(there, Linear(t(8, 64)).schedule(t(1, 2, 64)))
+    both = on(there, *ResidualNorm(RMSNorm(t(64))).schedule(t(2, 64), t(2, 64)))
+    for nodes in (product, both, product + both, both + product):
+        with pytest.raises(RatchetError, match="a node is on Device::GPU"):
+            Executable(here, nodes)
