@@ -1,7 +1,7 @@
 // 4-bit group-scaled weights (Q4_G32 / G64 / G128) x f16 or bf16 activations, 1..16 vectors: y[n][m] = sum_k (q - z) s x[n][k].
 //
 // A decode step reads every weight once: half a byte a weight and 3 / group for its scale and zero point bound it, next to
-// them the logic instructions that take the codes apart (half rate) and the warp MMAs (9 cycles each).
+// them the logic instructions that take the codes apart (half rate) and the warp MMAs (8 to 9 cycles each).
 //  * A warp takes a 16-row tile and a part of K in steps of 128 values; a CTA has a few tiles, all of the machine's resident at
 //    once where that is possible, and where rows are few its warps, then a cluster's CTAs, share K.  Codes go from global
 //    memory to registers, AHEAD steps asked for in advance, the first ones for constant weights before the kernel waits for
@@ -20,9 +20,10 @@
 //    at most by the count of additions, 2^-25 where it was looked for (codes at and next to zero points of 8 .. 31).  Beside f16's own
 //    rounding that shows in outputs 2^14 times smaller than their terms; a group of codes equal to its zero point adds as much, not 0.
 //
-// One vector, 51200 rows of 2560: 15.2 us with groups of 128 (4.5 TB/s), 16.6 of 64, 18.2 of 32; 2560 x 2560 3.7, the launch and two
-// trips to memory; 16 vectors 23.5 / 29 / 46: the epilogue of a group (FMAs by vectors, in pairs) and the masking bound those.  A
-// CUDA-core product of the same layout took 5 to 80 times as long (2560 x 10240 with 5 vectors: 841 us against 9.7).
+// One vector, 51200 rows of 2560: 15.4 us with groups of 128 (4.5 TB/s), 16.5 of 64, 18.2 of 32; 2560 x 2560 3.4, the launch and two
+// trips to memory; 16 vectors 23.5 / 29 / 46: the epilogue of a group (FMAs by vectors, in pairs), the masking, and the B operands' 21
+// thousand shared-memory wavefronts an SM bound those.  A CUDA-core product of the same layout took 5 to 90 times as long (2560 x 10240
+// with 5 vectors: 841 us against 9.5).
 #include <algorithm>
 
 #include "common.cuh"
@@ -128,7 +129,8 @@ __device__ __forceinline__ void spread_words(uint32_t (&w)[4], int t) {
 }
 
 // The dot product of one row and one vector again, element by element: an infinity among the activations makes q x - z x a NaN that
-// (q - z) x is not, so a NaN result is decided here by IEEE's rules for the plain sum.
+// (q - z) x is not, so a NaN result is decided here by IEEE's rules for the plain sum.  One thread does it: a NaN in every vector takes
+// 2560 x 2560 from 3.4 to 36 us, 51200 x 2560 with 16 vectors from 24 to 836.
 template <typename T> __device__ __noinline__ float exact_row(const MatmulParams &p, long long row, const T *x) {
     float acc = 0.f;
 #pragma unroll 1

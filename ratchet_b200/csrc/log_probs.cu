@@ -14,10 +14,11 @@
 //  * c is rounded as v log2(e) is not.  Rows so far from zero that this shows, and rows that never reach the first reference (f32's and
 //    bf16's lowest as a mask), take the differences v - max first, in a second pass.
 //
-// 2048 bf16 rows of 51865, 20 likeliest: 53 us, 4.0 TB/s; without the likeliest 40, 5.3 TB/s: 9.4 instructions a value at 2.9 a cycle
-// and SM, of them one exponential at 16 a cycle.  One f16 row 7.1 us: 4000 of 12000 cycles are the pass of one SM, the rest steps that
+// 2048 bf16 rows of 51865, 20 likeliest: 55 us, 3.9 TB/s, 11.5 instructions a value; without the likeliest 43.5, 4.9 TB/s, 8.9 at 2.8 a
+// cycle and SM, of them one exponential at 16 a cycle.  One f16 row 6.7 us: 4000 of 12000 cycles are the pass of one SM, the rest steps that
 // follow from one another (asking, sums and list, collecting from L2, ranking).  A pass for each of the maximum, the sums and every
-// likeliest token took 686 and 30 us.
+// likeliest token took 686 and 30 us.  Times that compare two forms below are of inputs that follow one another and half stay in L2:
+// 52 us for the first.
 #include <algorithm>
 
 #include "common.cuh"
@@ -67,7 +68,6 @@ template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     static constexpr int N = 4;
     static constexpr float START = -1e38f;
-    static constexpr uint32_t MINUS_INF = 0xff800000u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
     }
@@ -78,7 +78,6 @@ template <> struct Chunk<float> {
 template <> struct Chunk<__half> {
     static constexpr int N = 8;
     static constexpr float START = -94300.f; // the lowest's t: -204 (from -1e38 it was +inf, and every masked row went the long way below)
-    static constexpr uint32_t MINUS_INF = 0xfc00fc00u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -102,7 +101,6 @@ template <> struct Chunk<__half> {
 template <> struct Chunk<__nv_bfloat16> {
     static constexpr int N = 8;
     static constexpr float START = -1e38f;
-    static constexpr uint32_t MINUS_INF = 0xff80ff80u;
     static __device__ __forceinline__ void values(const uint4 &r, float (&v)[N]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -575,7 +573,7 @@ template <typename T, int TH> cudaError_t launch_threads(const rt_log_probs &op,
 
 template <typename T> cudaError_t launch_t(const rt_log_probs &op, int sm_count, cudaStream_t stream) {
     // Many rows: the work that a row costs beyond its values goes by its warps (2048 bf16 rows of 51865, 20 likeliest: 53 us with 256
-    // threads, 74 with 512; 200 f16 rows 17 and 12).  Few: more threads to a row, and a cluster's CTAs, then as many as have some four
+    // threads, 74 with 512, before both gained 1; 200 f16 rows 17 and 12).  Few: more threads to a row, and a cluster's CTAs, then as many as have some four
     // chunks a thread, only where a thread alone would have more than 32: two cluster barriers cost more than they save below that
     // (a row of 51865 f16 7.1 us, 8.0 as two CTAs; of 160000 11.5 alone, 10.4 as two, 8.7 as eight; 16 f32 rows of 51865 10.0, 11.8 as four).
     if (op.rows > 2LL * sm_count) return launch_threads<T, 256>(op, 1, stream);

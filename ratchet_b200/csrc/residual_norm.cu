@@ -8,10 +8,10 @@
 //  * Few rows: a thread per 16 bytes of the row, which asks for gate and weights together with the row instead of one after the other.
 //  * Longer rows: a CTA with more values a thread, or loops over the row, once per sum, that find it in L1 from the second pass on.
 //
-// 8192 bf16 rows of 2560, rms on both sides, a gate a sequence: 33.0 us, 5.1 TB/s (a CTA a row without the ring: 44; with means and
-// biases 44.8: four sums a row instead of two, 128 registers instead of 96).  What is left is instructions, 1.9 a cycle and SM with
-// 20 warps, and the start.  Rows of 2561, all off the 16-byte boundary, with a sixth warp for one value: 53 us.  One row: 3.4 us, the
-// launch.
+// 8192 bf16 rows of 2560, rms on both sides, a gate a sequence: 32.8 us, 5.1 TB/s (a CTA a row without the ring: 44; with means and
+// biases 43.8, a gate behind them 46.6: four sums a row instead of two, 128 registers instead of 96).  What is left is instructions,
+// 25 a value, 2.2 a cycle and SM with 20 warps, and the start.  Rows of 2561, all off the 16-byte boundary, with a sixth warp for one
+// value: 52.5 us.  One row: 2.5 us, the launch.
 #include <algorithm>
 #include <cfloat>
 #include <utility>
@@ -322,7 +322,7 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 // 16-byte words that hold the row are copied, which in the first and the last row would reach outside the tensor: those are read where
 // they are.  VEC = 1: the same copies for operands that differ in s, value by value.
 // Form: PLAIN has no means and no biases, which leaves the registers for more teams; GATED a gate behind a bias, where an infinite gate
-// may not be folded into both (8192 bf16 rows of 2560, layer norms, a gate a sequence: 46.8 us, 45.3 without that).
+// may not be folded into both (8192 bf16 rows of 2560, layer norms, a gate a sequence: 46.8 us, 45.3 without that, in turn).
 enum Form { PLAIN, MEANS, GATED };
 constexpr int N = 16, MAX_STAGES = 4, MAX_TEAMS = 8, WALK_SMEM = 200 * 1024;
 constexpr int MIN_WALK_D = 8; // 16 bytes: the words of a row that is neither first nor last lie in the tensor
