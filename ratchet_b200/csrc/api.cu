@@ -1141,7 +1141,8 @@ static rt_status launch_node(rt_plan *plan, const void *lhs, const void *rhs, co
         if (opts->n_out > RT_MAX_PEERS || opts->out_col < 0 || opts->out_ld < opts->out_col + plan->S)
             return fail(RT_ERR_ARG, "rt_matmul_launch_ex: bad scatter description");
         for (int d = 0; d < opts->n_out; d++)
-            if (!opts->outs[d]) return fail(RT_ERR_ARG, "rt_matmul_launch_ex: null scatter destination");
+            if (!opts->outs[d] || misaligned(opts->outs[d], plan->spec.out_dt))
+                return fail(RT_ERR_ARG, "rt_matmul_launch_ex: a scatter destination is null or not aligned to its elements");
     }
     const Spec &s = plan->spec;
     if (scatter && s.epilogue == RT_EPILOGUE_SILU_MUL)

@@ -253,6 +253,38 @@ def test_infinite_gates_do_the_same_to_few_rows_and_to_many(d, post, dt, gpu):
             assert x is None or np.isnan(x.resolve().to(Device.CPU).to_f32()).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("d", [96, 383, 520, 1003])
+def test_infinite_gates_of_some_rows_only(d, dt, gpu):
+    """A gate per row and per sequence, infinite at a few places of a few of them, behind a layer norm with a bias: teams cross from
+    ordinary gates to those and back."""
+    rng = np.random.default_rng(93)
+    shape = (60, 7, 9, d)
+    r, y = (round_to(dt, rng.standard_normal(shape, dtype=np.float32)) for _ in range(2))
+    w, b = round_to(dt, rng.uniform(0.5, 2.0, d).astype(np.float32)), round_to(dt, rng.uniform(-2.0, 2.0, d).astype(np.float32))
+    t = lambda a: Tensor.from_data(a, gpu, dt)  # noqa: E731
+    mod = ResidualNorm(RMSNorm(t(w)), LayerNorm(t(w), t(b)))
+    truth, pre = ("layer", w.astype(np.float64), b.astype(np.float64), np.float64(np.float32(1e-5))), ("rms", w.astype(np.float64), 0.0, np.float64(np.float32(1e-5)))
+    for lead in ((60, 7, 9), (60, 1, 1)):
+        gate = round_to(dt, rng.uniform(0.5, 1.5, (*lead, d)).astype(np.float32))
+        rows = gate.reshape(-1, d)
+        for i in rng.choice(len(rows), max(3, len(rows) // 20), replace=False):
+            rows[i, rng.integers(d)] = rng.choice([np.inf, -np.inf])
+        h, x = mod.schedule(t(r), t(y), t(gate))
+        h, x = (v.resolve().to(Device.CPU).to_f32().astype(np.float64) for v in (h, x))
+        finite = np.broadcast_to(np.isfinite(gate), shape)
+        with np.errstate(invalid="ignore"):
+            th, tx = norm_truth(r.astype(np.float64), y.astype(np.float64), np.where(np.isfinite(gate), gate, 1.0).astype(np.float64), truth, pre, 1.0, 1.0)
+            u, eu = norm_truth(None, y.astype(np.float64), None, truth, (None, 1, 0, 0), 1.0, 1.0)[0]
+            want = np.where(finite, 0.0, gate.astype(np.float64) * u)
+            ok = np.where(finite, close(h, th, dt), (h == want) | (np.abs(u) <= 2 * eu))
+            assert np.all(ok)
+            whole = finite.all(-1)
+            # an infinite value's row has a root mean square of inf: 0 for what is finite, NaN for inf / inf
+            assert np.all(close(x, tx, dt)[whole]) and np.all(np.where(finite, x == 0, np.isnan(x))[~whole])
+
+
 # ------------------------------------------------------------------------------------------------ CPU: executables
 
 def test_an_executable_refuses_nodes_of_another_device():

@@ -1,4 +1,6 @@
 """4-bit group weights where they can go wrong: addresses, cancellation, activations that are not finite."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -62,3 +64,19 @@ def test_codes_at_their_zero_point(zero, near, dt, act, gpu):
         got = out.resolve().to(Device.CPU).to_f32()
         over = np.abs(got[0] - y) - apart_bound(act, dt, q, s, z, x[0], y)
         assert np.all(over <= 0), (m, k, rows, float(over.max()))
+
+
+@pytest.mark.gpu
+def test_scatter_destinations_inside_an_element_are_refused(gpu):
+    lib, m, k, rows = _lib.load(), 256, 256, 64
+    plan = gpu.plan_for(Linear(Tensor((m, k), G64, gpu)).schedule(Tensor((1, rows, k), F16, gpu)).op.desc)
+    assert "umma" in lib.rt_plan_kernel(plan).decode()
+    store = rb.GpuBuffer(gpu, 1 << 18)
+    zero = np.zeros(1 << 18, np.uint8)
+    _lib.check(lib.rt_upload(gpu._h, store._h, 0, zero.ctypes.data, zero.size, 1))
+    opts = _lib.rt_launch_opts()
+    opts.n_out, opts.out_ld, opts.out_col = 1, m, 0
+    for off, want in ((0, _lib.RT_OK), (1, _lib.RT_ERR_ARG)):
+        opts.outs[0] = store.ptr + (1 << 17) + off
+        assert lib.rt_matmul_launch_ex(plan, store.ptr, store.ptr + 65536, None, None, None, ctypes.byref(opts)) == want
+    gpu.sync()
