@@ -573,9 +573,10 @@ template <typename T, int TH> cudaError_t launch_threads(const rt_log_probs &op,
 
 template <typename T> cudaError_t launch_t(const rt_log_probs &op, int sm_count, cudaStream_t stream) {
     // Many rows: the work that a row costs beyond its values goes by its warps (2048 bf16 rows of 51865, 20 likeliest: 53 us with 256
-    // threads, 74 with 512, before both gained 1; 200 f16 rows 17 and 12).  Few: more threads to a row, and a cluster's CTAs, then as many as have some four
-    // chunks a thread, only where a thread alone would have more than 32: two cluster barriers cost more than they save below that
-    // (a row of 51865 f16 7.1 us, 8.0 as two CTAs; of 160000 11.5 alone, 10.4 as two, 8.7 as eight; 16 f32 rows of 51865 10.0, 11.8 as four).
+    // threads, 74 with 512, before both gained 1; 200 f16 rows 17 and 12).  Few: more threads to a row, and a cluster's CTAs, then as many
+    // as have some four chunks a thread, only where a thread alone would have more than 32: two cluster barriers cost more than they save
+    // below that (a row of 51865 f16 7.1 us, 8.0 as two CTAs; of 160000 11.5 alone, 10.4 as two, 8.7 as eight; 16 f32 rows of 51865 10.0,
+    // 11.8 as four).
     if (op.rows > 2LL * sm_count) return launch_threads<T, 256>(op, 1, stream);
     int ranks = 1;
     while (ranks < MAX_RANKS && op.rows * ranks * 2 <= 2LL * sm_count && op.vocab / Chunk<T>::N > (ranks == 1 ? 32LL : 4LL) * ranks * 512) ranks *= 2;
